@@ -388,6 +388,55 @@ MIXFP4_API int mixfp4_gemm_h128_static(const void* x, int64_t m, int64_t ldx,
                 const float* global_scale, int64_t n, int64_t k, int layout, const void* lut,
                 void* y, int out_dtype, int64_t ldy, int* status, void* stream);
 
+/* Block-scaled FP8 (no reference counterpart: the reference leaves the layers that four bits hurt in bf16).  E4M3 codes with
+ * one fp32 scale per block: activations per row and 128 columns, weights per 128 x 128 tile.  scale = largest magnitude of
+ * the block / 448 (1 where that is zero), code = e4m3(fp32(value / scale)), ties to even.  A block that holds a value that is
+ * not finite gets such a scale, and the results that read it are NaN.
+ * mixfp4_fp8_scale_rows(m): rows that a scale array of m rows of activations has room for (m rounded up to 128).
+ * mixfp4_fp8_quantize_rows: x [m, k] (any element type, row stride ldx) -> codes [m, ldq], zero from k to kpad, and scales
+ *   [ceil(k/128)][lds], the scale of (row, block) at block * lds + row; lds >= mixfp4_fp8_scale_rows(m); rows m.. stay as they were.
+ * mixfp4_fp8_quantize_tiles: w [n, k] -> codes [n, ldq] likewise, scales [ceil(n/128)][ceil(k/128)].
+ * codes and scales 16-byte aligned (scales of tiles 4), ldq >= mixfp4_padded_k(k) and a multiple of 16, lds a multiple of 4.
+ * mixfp4_fp8_dequant: y[r, c] = code * scale[r / rows_per_scale * row_stride + c / 128 * block_stride], rounded once;
+ *   rows_per_scale 1 or 128. */
+MIXFP4_API int64_t mixfp4_fp8_scale_rows(int64_t m);
+MIXFP4_API int mixfp4_fp8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx, uint8_t* codes,
+                             int64_t ldq, float* scales, int64_t lds, void* stream);
+MIXFP4_API int mixfp4_fp8_quantize_tiles(const void* w, int dtype, int64_t n, int64_t k, int64_t ldw, uint8_t* codes,
+                              int64_t ldq, float* scales, void* stream);
+MIXFP4_API int mixfp4_fp8_dequant(const uint8_t* codes, int64_t ldq, const float* scales, int64_t row_stride,
+                       int64_t block_stride, int rows_per_scale, int64_t rows, int64_t k, void* y, int out_dtype,
+                       int64_t ldy, void* stream);
+
+/* y[m, n] = sum over blocks b of x_scales[b][m] * w_scales[n / 128][b] * (sum over k in b of x[m, k] w[n, k]), E4M3 products
+ * summed in fp32, one rounding to out_dtype (bf16, f16 or fp32).  Codes: rows of k bytes, 16-byte aligned, ldx and ldw
+ * multiples of 16; what lies behind k in a row is not read.  x_scales as mixfp4_fp8_quantize_rows lays them out (the pad rows
+ * are read, their values do not matter).  status as in mixfp4_gemm.
+ * mixfp4_fp8_linear: the same with x still dense: quantized into the workspace (at least
+ * mixfp4_fp8_workspace_bytes(m, k) bytes, 16-byte aligned), then multiplied, the product starting under the quantizer's tail. */
+MIXFP4_API int mixfp4_fp8_gemm(const uint8_t* x, int64_t ldx, const float* x_scales, int64_t lds, const uint8_t* w,
+                    int64_t ldw, const float* w_scales, int64_t m, int64_t n, int64_t k, void* y, int out_dtype,
+                    int64_t ldy, int* status, void* stream);
+MIXFP4_API int64_t mixfp4_fp8_workspace_bytes(int64_t m, int64_t k);
+MIXFP4_API int mixfp4_fp8_linear(const void* x, int dtype, int64_t m, int64_t ldx, const uint8_t* w, int64_t ldw,
+                      const float* w_scales, int64_t n, int64_t k, void* y, int out_dtype, int64_t ldy,
+                      void* workspace, int64_t workspace_bytes, int* status, void* stream);
+
+/* One token a row from logits [rows, vocab] (row stride ld) and random numbers uniform[rows] in [0, 1) (no reference
+ * counterpart: the reference generates no tokens).  w_i = exp((x_i - max) / temperature); kept are, in the order of falling
+ * values (equal ones by index), the first top_k, of those the shortest run whose weights reach top_p of theirs, of those
+ * every w_i >= min_p; token = the first index in the vocabulary's order at which the kept weights add up to more than
+ * uniform * their sum.  Each setting is an array with a value for every row, or NULL and a value for all.  temperature
+ * <= 0: the first of the largest logits; top_k <= 0 or >= vocab, top_p >= 1, min_p <= 0: no such filter.  Logits of -inf and NaN
+ * are never chosen, a row of nothing else gives -1.  logprob (optional): log of the token's share of the kept weights, -inf
+ * beside -1.  Weights count in multiples of 2^-44 of the largest.  No workspace.  MIXFP4_E_TOO_LARGE beyond
+ * mixfp4_sample_max_vocab() columns. */
+MIXFP4_API int64_t mixfp4_sample_max_vocab(void);
+MIXFP4_API int mixfp4_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const float* uniform,
+                  const float* temperature, double temperature_all, const int* top_k, int top_k_all,
+                  const float* top_p, double top_p_all, const float* min_p, double min_p_all, int64_t* token,
+                  float* logprob, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,6 +10,9 @@ from .quant import (E0M3_LEVELS, E2M1_LEVELS, SCALE_GROUP_SIZE, CandidateBlocks,
                     ScaledCandidate, build_candidates, build_scaled_candidate, dequantize, fake_quantize_activations, quantize_e0m3, quantize_e2m1, packed_nbytes, quant_mixfp4_granularity, quantize_packed, tensor_amax)
 from .rotation import TRANSFORM_BANK, TransformSpec, apply_transform, get_transform
 from .linear import MixFP4Linear, decode_status, gemm_status, mixfp4_linear, mixfp4_linear_grouped
+from .fp8 import (FP8Activations, FP8Linear, FP8Weight, dequantize_fp8, fp8_linear, quantize_fp8_activations,
+                  quantize_fp8_weight)
+from .sampling import sample_logits
 from .convert import load_packed, named_linears, quantize_model_weights, save_packed
 
 __all__ = [
@@ -17,5 +20,6 @@ __all__ = [
     "quantize_e0m3", "quantize_e2m1", "PackedWeight", "dequantize",
     "fake_quantize_activations", "packed_nbytes", "quant_mixfp4_granularity", "quantize_packed", "tensor_amax", "TRANSFORM_BANK",
     "TransformSpec", "apply_transform", "get_transform", "MixFP4Linear", "decode_status", "gemm_status", "mixfp4_linear", "mixfp4_linear_grouped",
-    "load_packed", "named_linears", "quantize_model_weights", "save_packed",
+    "FP8Activations", "FP8Linear", "FP8Weight", "dequantize_fp8", "fp8_linear", "quantize_fp8_activations", "quantize_fp8_weight",
+    "sample_logits", "load_packed", "named_linears", "quantize_model_weights", "save_packed",
 ]

@@ -142,6 +142,25 @@ def _declare(h: ctypes.CDLL) -> None:
     h.mixfp4_gemm_h128_static_max_bytes.argtypes = []
     h.mixfp4_gemm_h128_static.restype = i32
     h.mixfp4_gemm_h128_static.argtypes = [p, i64, i64, p, p, p, p, i64, i64, i32, p, p, i32, i64, p, p]
+    f64 = ctypes.c_double
+    h.mixfp4_fp8_scale_rows.restype = i64
+    h.mixfp4_fp8_scale_rows.argtypes = [i64]
+    h.mixfp4_fp8_quantize_rows.restype = i32
+    h.mixfp4_fp8_quantize_rows.argtypes = [p, i32, i64, i64, i64, p, i64, p, i64, p]
+    h.mixfp4_fp8_quantize_tiles.restype = i32
+    h.mixfp4_fp8_quantize_tiles.argtypes = [p, i32, i64, i64, i64, p, i64, p, p]
+    h.mixfp4_fp8_dequant.restype = i32
+    h.mixfp4_fp8_dequant.argtypes = [p, i64, p, i64, i64, i32, i64, i64, p, i32, i64, p]
+    h.mixfp4_fp8_gemm.restype = i32
+    h.mixfp4_fp8_gemm.argtypes = [p, i64, p, i64, p, i64, p, i64, i64, i64, p, i32, i64, p, p]
+    h.mixfp4_fp8_workspace_bytes.restype = i64
+    h.mixfp4_fp8_workspace_bytes.argtypes = [i64, i64]
+    h.mixfp4_fp8_linear.restype = i32
+    h.mixfp4_fp8_linear.argtypes = [p, i32, i64, i64, p, i64, p, i64, i64, p, i32, i64, p, i64, p, p]
+    h.mixfp4_sample_max_vocab.restype = i64
+    h.mixfp4_sample_max_vocab.argtypes = []
+    h.mixfp4_sample.restype = i32
+    h.mixfp4_sample.argtypes = [p, i32, i64, i64, i64, p, p, f64, p, i32, p, f64, p, f64, p, p, p]
 
 
 # every symbol include/mixfp4_b200.h declares
@@ -154,6 +173,8 @@ EXPORTED = (
     "mixfp4_comm_buffer_bytes", "mixfp4_comm_buffer", "mixfp4_comm_open_local", "mixfp4_comm_destroy",
     "mixfp4_gemv_allreduce", "mixfp4_set_wait_limit_ns", "mixfp4_check_status",
     "mixfp4_gemm_workspace_bytes", "mixfp4_gemm", "mixfp4_gemm_grouped", "mixfp4_gemm_a4", "mixfp4_gemm_h128_static_max_bytes", "mixfp4_gemm_h128_static",
+    "mixfp4_fp8_scale_rows", "mixfp4_fp8_quantize_rows", "mixfp4_fp8_quantize_tiles", "mixfp4_fp8_dequant", "mixfp4_fp8_gemm",
+    "mixfp4_fp8_workspace_bytes", "mixfp4_fp8_linear", "mixfp4_sample_max_vocab", "mixfp4_sample",
 )
 
 

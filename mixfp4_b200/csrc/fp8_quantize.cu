@@ -1,0 +1,247 @@
+// E4M3 codes with one fp32 scale per block of 128: the operands of the block-scaled product (fp8_gemm.cu).
+//   activations  s[m, b] = max |x[m, 128 b ..]| / 448, a scale for every row and 128 columns
+//   weights      s[i, b] = max |w[128 i .., 128 b ..]| / 448, a scale for every 128 x 128 tile
+//   codes        q = e4m3(x / s): the fp32 quotient, then the nearest E4M3 value (ties to even)
+// The scale is held in fp32; one that would be zero (a block of zeros, or of magnitudes below 448 times the smallest
+// subnormal) becomes 1.  A block that holds a NaN or an infinity has that as its scale, and NaN codes.
+//
+// Both passes read a block once, keep it in registers and write codes and scale from there: bound by HBM.
+
+#include "common.cuh"
+#include "fp8.cuh"
+
+namespace mixfp4 {
+namespace {
+
+constexpr float kLargest = 448.0f;
+constexpr int kLaneElems = 16, kLanesPerRow = kFp8Block / kLaneElems;       // a lane holds 16 elements of a row's block
+
+// The larger magnitude, NaN if either is one (fmaxf would drop it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// 16 consecutive elements of a row from column c, zero past k.
+template <typename T>
+__device__ __forceinline__ void load16(const T* row, int64_t c, int64_t k, bool vec, float (&v)[kLaneElems]) {
+    if (vec && c + kLaneElems <= k) {
+        constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kLaneElems / kPer; ++i) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+            const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) v[i * kPer + j] = Elem<T>::load(e + j);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kLaneElems; ++j) v[j] = c + j < k ? Elem<T>::load(row + c + j) : 0.0f;
+    }
+}
+
+__device__ __forceinline__ float largest_of(const float (&v)[kLaneElems]) {
+    float a = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kLaneElems; ++j) a = max_nan(a, fabsf(v[j]));
+    return a;
+}
+
+__device__ __forceinline__ float block_scale(float largest) {
+    const float s = __fdiv_rn(largest, kLargest);
+    return s == 0.0f ? 1.0f : s;
+}
+
+// x / s rounded once, for the 16 values of a lane.  One reciprocal for all of them and a residual step each:
+// q = x r, then q + (x - q s) r, which is the rounded quotient when r is the rounded reciprocal and nothing
+// underflows (Markstein 1990, theorem on final rounding).  Scales outside 2^+-100 take the division itself.
+__device__ __forceinline__ uint4 encode16(const float (&v)[kLaneElems], float s) {
+    float q[kLaneElems];
+    if (s > 0x1p-100f && s < 0x1p100f) {
+        const float r = __frcp_rn(s);
+#pragma unroll
+        for (int j = 0; j < kLaneElems; ++j) {
+            const float q0 = __fmul_rn(v[j], r);
+            q[j] = __fmaf_rn(__fmaf_rn(-q0, s, v[j]), r, q0);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kLaneElems; ++j) q[j] = __fdiv_rn(v[j], s);
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[4 * i], q[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[4 * i + 2], q[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
+        w[i] = lo | (hi << 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A group of eight lanes per row and block.  scales: [block][lds], a row's scales a column of it, so that the product reads
+// the scales of neighbouring rows together.
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_rows_kernel(const T* x, int64_t m, int64_t k, int64_t ldx, bool vec,
+                                                       uint8_t* codes, int64_t ldq, float* scales, int64_t lds) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");                       // x may be the kernel before's output
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int64_t blocks = (k + kFp8Block - 1) / kFp8Block, total = m * blocks;
+    const int sub = threadIdx.x % kLanesPerRow;
+    const int64_t stride = (int64_t)gridDim.x * (blockDim.x / kLanesPerRow);
+    for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / kLanesPerRow) + threadIdx.x / kLanesPerRow;; i += stride) {
+        const bool in = i < total;
+        if (!__any_sync(0xffffffffu, in)) break;
+        const int64_t row = in ? i / blocks : 0, b = in ? i - row * blocks : 0;
+        const int64_t c = b * kFp8Block + sub * kLaneElems;
+        float v[kLaneElems];
+        load16(x + row * ldx, c, in ? k : 0, vec, v);
+        float a = largest_of(v);
+#pragma unroll
+        for (int d = 1; d < kLanesPerRow; d *= 2) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, d));
+        if (in) {
+            const float s = block_scale(a);
+            *reinterpret_cast<uint4*>(codes + row * ldq + c) = encode16(v, s);
+            if (sub == 0) scales[b * lds + row] = s;
+        }
+    }
+}
+
+// A CTA of 512 threads per 128 x 128 tile: 64 rows a pass, two passes, 32 elements a thread.
+constexpr int kTileThreads = 512, kTilePasses = 128 * kLanesPerRow / kTileThreads;
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads) fp8_tiles_kernel(const T* w, int64_t n, int64_t k, int64_t ldw, bool vec,
+                                                                 uint8_t* codes, int64_t ldq, float* scales) {
+    __shared__ float warp_max[kTileThreads / 32];
+    const int64_t blocks = (k + kFp8Block - 1) / kFp8Block;
+    const int64_t tile = blockIdx.x / blocks, b = blockIdx.x - tile * blocks;
+    const int sub = threadIdx.x % kLanesPerRow, first = threadIdx.x / kLanesPerRow;
+    const int64_t c = b * kFp8Block + sub * kLaneElems;
+    float v[kTilePasses][kLaneElems];
+    float a = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kTilePasses; ++p) {
+        const int64_t row = tile * kFp8Block + first + p * (kTileThreads / kLanesPerRow);
+        load16(w + (row < n ? row : 0) * ldw, c, row < n ? k : 0, vec, v[p]);
+        a = max_nan(a, largest_of(v[p]));
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, d));
+    if (threadIdx.x % 32 == 0) warp_max[threadIdx.x / 32] = a;
+    __syncthreads();
+    a = warp_max[0];
+#pragma unroll
+    for (int i = 1; i < kTileThreads / 32; ++i) a = max_nan(a, warp_max[i]);
+    const float s = block_scale(a);
+    if (threadIdx.x == 0) scales[tile * blocks + b] = s;
+#pragma unroll
+    for (int p = 0; p < kTilePasses; ++p) {
+        const int64_t row = tile * kFp8Block + first + p * (kTileThreads / kLanesPerRow);
+        if (row < n) *reinterpret_cast<uint4*>(codes + row * ldq + c) = encode16(v[p], s);
+    }
+}
+
+// y = code * scale, rounded once.  One thread per 4 columns.
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_dequant_kernel(const uint8_t* codes, int64_t ldq, const float* scales,
+                                                          int64_t row_stride, int64_t block_stride, int rows_per_scale,
+                                                          int64_t rows, int64_t k, T* y, int64_t ldy) {
+    const int64_t quads = (k + 3) / 4, total = rows * quads;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t row = i / quads, c = (i - row * quads) * 4;
+        const float s = __ldg(scales + row / rows_per_scale * row_stride + c / kFp8Block * block_stride);
+        for (int j = 0; j < 4 && c + j < k; ++j)
+            y[row * ldy + c + j] = Elem<T>::round(__fmul_rn(e4m3_to_float(codes[row * ldq + c + j]), s));
+    }
+}
+
+template <typename F>
+int by_type(int dtype, F&& f) {
+    switch (dtype) {
+        case MIXFP4_BF16: return f(__nv_bfloat16());
+        case MIXFP4_F16: return f(__half());
+        case MIXFP4_F32: return f(float());
+        default: return MIXFP4_E_DTYPE;
+    }
+}
+int elem_bytes(int dtype) { return dtype == MIXFP4_F32 ? 4 : 2; }
+constexpr int64_t kMaxSide = 0x7fffffff;          // a tensor map's coordinates are 32-bit
+
+}  // namespace
+
+int fp8_check_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx, const uint8_t* codes, int64_t ldq,
+                   const float* scales, int64_t lds) {
+    if (!x || !codes || !scales) return MIXFP4_E_NULL;
+    if (dtype != MIXFP4_BF16 && dtype != MIXFP4_F16 && dtype != MIXFP4_F32) return MIXFP4_E_DTYPE;
+    if (m <= 0 || k <= 0 || m > kMaxSide || k > kMaxSide - 128 || ldx < k || ldq < padded_k(k) || lds < fp8_scale_rows(m))
+        return MIXFP4_E_SHAPE;
+    if (!aligned(codes, 16) || ldq % 16 != 0 || !aligned(scales, 16) || lds % 4 != 0) return MIXFP4_E_ALIGN;
+    return MIXFP4_OK;
+}
+
+int fp8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx, uint8_t* codes, int64_t ldq,
+                      float* scales, int64_t lds, cudaStream_t st) {
+    return by_type(dtype, [&](auto t) -> int {
+        using T = decltype(t);
+        const bool vec = aligned(x, 16) && ldx * (int64_t)sizeof(T) % 16 == 0;
+        const int64_t groups = m * ((k + kFp8Block - 1) / kFp8Block), per_cta = 256 / kLanesPerRow;
+        const int64_t ctas = (groups + per_cta - 1) / per_cta;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(ctas < 148 * 64 ? ctas : 148 * 64));
+        cfg.blockDim = dim3(256);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        MIXFP4_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fp8_rows_kernel<T>, static_cast<const T*>(x), m, k, ldx, vec, codes, ldq,
+                                             scales, lds));
+        return check_launch("fp8_rows_kernel");
+    });
+}
+
+}  // namespace mixfp4
+
+using namespace mixfp4;
+
+extern "C" int64_t mixfp4_fp8_scale_rows(int64_t m) { return m <= 0 ? 0 : fp8_scale_rows(m); }
+
+extern "C" int mixfp4_fp8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx, uint8_t* codes,
+                                        int64_t ldq, float* scales, int64_t lds, void* stream) {
+    if (const int rc = fp8_check_rows(x, dtype, m, k, ldx, codes, ldq, scales, lds)) return rc;
+    return fp8_quantize_rows(x, dtype, m, k, ldx, codes, ldq, scales, lds, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mixfp4_fp8_quantize_tiles(const void* w, int dtype, int64_t n, int64_t k, int64_t ldw, uint8_t* codes,
+                                         int64_t ldq, float* scales, void* stream) {
+    if (!w || !codes || !scales) return MIXFP4_E_NULL;
+    if (dtype != MIXFP4_BF16 && dtype != MIXFP4_F16 && dtype != MIXFP4_F32) return MIXFP4_E_DTYPE;
+    if (n <= 0 || k <= 0 || n > kMaxSide - 128 || k > kMaxSide - 128 || ldw < k || ldq < padded_k(k)) return MIXFP4_E_SHAPE;
+    const int64_t tiles = (n + kFp8Block - 1) / kFp8Block * ((k + kFp8Block - 1) / kFp8Block);
+    if (tiles > kMaxSide) return MIXFP4_E_SHAPE;
+    if (!aligned(codes, 16) || ldq % 16 != 0 || !aligned(scales, 4)) return MIXFP4_E_ALIGN;
+    const bool vec = aligned(w, 16) && ldw * elem_bytes(dtype) % 16 == 0;
+    return by_type(dtype, [&](auto t) -> int {
+        using T = decltype(t);
+        fp8_tiles_kernel<T><<<(unsigned)tiles, kTileThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+            static_cast<const T*>(w), n, k, ldw, vec, codes, ldq, scales);
+        return check_launch("fp8_tiles_kernel");
+    });
+}
+
+extern "C" int mixfp4_fp8_dequant(const uint8_t* codes, int64_t ldq, const float* scales, int64_t row_stride,
+                                  int64_t block_stride, int rows_per_scale, int64_t rows, int64_t k, void* y, int out_dtype,
+                                  int64_t ldy, void* stream) {
+    if (!codes || !scales || !y) return MIXFP4_E_NULL;
+    if (rows_per_scale != 1 && rows_per_scale != kFp8Block) return MIXFP4_E_MODE;
+    if (rows <= 0 || k <= 0 || rows > kMaxSide || k > kMaxSide || ldq < k || ldy < k || row_stride < 0 || block_stride < 0)
+        return MIXFP4_E_SHAPE;
+    return by_type(out_dtype, [&](auto t) -> int {
+        using T = decltype(t);
+        const int64_t ctas = (rows * ((k + 3) / 4) + 255) / 256;
+        fp8_dequant_kernel<T><<<(unsigned)(ctas < 148 * 64 ? ctas : 148 * 64), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+            codes, ldq, scales, row_stride, block_stride, rows_per_scale, rows, k, static_cast<T*>(y), ldy);
+        return check_launch("fp8_dequant_kernel");
+    });
+}

@@ -1,0 +1,254 @@
+"""Block-scaled FP8: the linear for layers that four bits hurt (output heads, sensitive projections), at half the bytes of bf16.
+
+    activations   E4M3 codes and one fp32 scale for every row and 128 columns
+    weights       E4M3 codes and one fp32 scale for every 128 x 128 tile
+    scale         the block's largest magnitude / 448 (1 where that is zero); code = e4m3(fp32(value / scale))
+    y[m, n]     = sum over blocks b of sx[m, b] * sw[n // 128, b] * (sum of code products in b), in fp32, rounded once
+
+The reference keeps such layers in bf16 (project_quant/modeling.py:65-68 leaves output heads out of the walk); there is no
+counterpart of this format in it.  Inputs that are not finite make their block's scale, and the results that read it, NaN.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+from torch import nn
+
+from . import _native as nat
+from .linear import _status_word
+
+FP8_BLOCK = 128
+_OUT_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _blocks(size: int) -> int:
+    return -(-size // FP8_BLOCK)
+
+
+def _codes_for_kernels(codes: torch.Tensor) -> torch.Tensor:
+    """The codes with rows that a tensor map can address (16-byte aligned); themselves where they are so already."""
+    rows, k = codes.shape
+    if codes.stride(1) == 1 and codes.stride(0) >= k and codes.stride(0) % 16 == 0 and codes.data_ptr() % 16 == 0:
+        return codes
+    held = torch.empty((rows, _blocks(k) * FP8_BLOCK), dtype=codes.dtype, device=codes.device)[:, :k]
+    held.copy_(codes)
+    return held
+
+
+def _check_parts(codes: torch.Tensor, scales: torch.Tensor, rows_per_scale: int) -> torch.Tensor:
+    if codes.dtype == torch.uint8:
+        codes = codes.view(torch.float8_e4m3fn)
+    if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        raise TypeError("codes must be float8_e4m3fn (or its bytes), scales float32")
+    if codes.ndim != 2 or 0 in codes.shape:
+        raise ValueError("codes must be a matrix with at least one row and column")
+    want = (-(-codes.shape[0] // rows_per_scale), _blocks(codes.shape[1]))
+    if tuple(scales.shape) != want:
+        raise ValueError(f"scales must have the shape {want}, one for each block of the codes, not {tuple(scales.shape)}")
+    if codes.device != scales.device:
+        raise ValueError("codes and scales must be on the same device")
+    return codes
+
+
+@dataclass
+class FP8Weight:
+    """A quantized [n, k] weight: codes float8_e4m3fn [n, k] with 16-byte aligned rows, scales float32 [ceil(n/128), ceil(k/128)]."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self):
+        self.n, self.k = self.codes.shape
+
+    @classmethod
+    def from_tensors(cls, codes: torch.Tensor, scales: torch.Tensor) -> "FP8Weight":
+        """Codes (float8_e4m3fn or their bytes) and scales of a checkpoint; copied only where their rows are not aligned."""
+        codes = _check_parts(codes, scales, FP8_BLOCK)
+        return cls(_codes_for_kernels(codes), scales.contiguous())
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return self.n * self.k + self.scales.numel() * 4
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        return dequantize_fp8(self, dtype)
+
+    def to(self, device) -> "FP8Weight":
+        return FP8Weight.from_tensors(self.codes.to(device), self.scales.to(device))
+
+
+@dataclass
+class FP8Activations:
+    """Quantized rows: codes float8_e4m3fn [m, k]; scales float32 [m, ceil(k/128)], a view whose columns are contiguous and
+    padded to 128 rows (what the product fetches).  `shape` and `dtype` are the source's."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    shape: torch.Size
+    dtype: torch.dtype
+
+    @classmethod
+    def from_tensors(cls, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> "FP8Activations":
+        codes = _check_parts(codes, scales, 1)
+        held = _scale_room(codes.shape[0], codes.shape[1], codes.device)
+        held.copy_(scales)
+        return cls(_codes_for_kernels(codes), held, codes.shape, dtype)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        return dequantize_fp8(self, self.dtype if dtype is None else dtype).reshape(self.shape)
+
+
+def _scale_room(m: int, k: int, device) -> torch.Tensor:
+    return torch.empty((_blocks(k), _blocks(m) * FP8_BLOCK), dtype=torch.float32, device=device).t()[:m]
+
+
+def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
+    """[..., K] as rows with unit stride along K and a row stride of at least K."""
+    nat.require_cuda(x, what)
+    if x.dtype not in nat.DTYPE_CODE:
+        raise TypeError(f"{what} must be bfloat16, float16 or float32")
+    if x.ndim == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{what} must have at least one column")
+    x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1 or x2.stride(0) < x2.shape[1]:
+        x2 = x2.reshape(1, -1) if x2.shape[0] == 1 and x2.stride(1) == 1 else x2.contiguous()
+        if x2.stride(0) < x2.shape[1]:                   # a single row, whose stride can be any number
+            x2 = x2.as_strided(x2.shape, (x2.shape[1], 1))
+    return x2
+
+
+@torch.no_grad()
+def quantize_fp8_weight(w: torch.Tensor) -> FP8Weight:
+    """A dense [n, k] weight (bf16, f16 or fp32, on the GPU) to codes and a scale for every 128 x 128 tile, in one pass."""
+    if w.ndim != 2 or 0 in w.shape:
+        raise ValueError("the weight must be a matrix with at least one row and column")
+    w = _rows(w.detach(), "the weight")
+    n, k = w.shape
+    codes = torch.empty((n, _blocks(k) * FP8_BLOCK), dtype=torch.float8_e4m3fn, device=w.device)
+    scales = torch.empty((_blocks(n), _blocks(k)), dtype=torch.float32, device=w.device)
+    with nat.on_device(w.device):
+        st = nat.lib().mixfp4_fp8_quantize_tiles(w.data_ptr(), nat.DTYPE_CODE[w.dtype], n, k, w.stride(0), codes.data_ptr(),
+                                                 codes.stride(0), scales.data_ptr(), nat.stream_ptr(w.device))
+    nat.check("mixfp4_fp8_quantize_tiles", st)
+    return FP8Weight(codes[:, :k], scales)
+
+
+@torch.no_grad()
+def quantize_fp8_activations(x: torch.Tensor) -> FP8Activations:
+    """Rows [..., K] to codes and a scale for every row and 128 columns: once for all the weights that read them."""
+    x2 = _rows(x.detach(), "x")
+    m, k = x2.shape
+    codes = torch.empty((m, _blocks(k) * FP8_BLOCK), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = _scale_room(m, k, x.device)
+    if m:
+        with nat.on_device(x.device):
+            st = nat.lib().mixfp4_fp8_quantize_rows(x2.data_ptr(), nat.DTYPE_CODE[x.dtype], m, k, x2.stride(0), codes.data_ptr(),
+                                                    codes.stride(0), scales.data_ptr(), _blocks(m) * FP8_BLOCK,
+                                                    nat.stream_ptr(x.device))
+        nat.check("mixfp4_fp8_quantize_rows", st)
+    return FP8Activations(codes[:, :k], scales, x.shape, x.dtype)
+
+
+@torch.no_grad()
+def dequantize_fp8(q: FP8Weight | FP8Activations, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """code * scale as a dense matrix, rounded once."""
+    if dtype not in nat.DTYPE_CODE:
+        raise TypeError("dtype must be bfloat16, float16 or float32")
+    nat.require_cuda(q.codes, "codes")
+    rows, k = q.codes.shape
+    out = torch.empty((rows, k), dtype=dtype, device=q.device)
+    if rows:
+        with nat.on_device(q.device):
+            st = nat.lib().mixfp4_fp8_dequant(q.codes.data_ptr(), q.codes.stride(0), q.scales.data_ptr(), q.scales.stride(0),
+                                              q.scales.stride(1), FP8_BLOCK if isinstance(q, FP8Weight) else 1, rows, k,
+                                              out.data_ptr(), nat.DTYPE_CODE[dtype], k, nat.stream_ptr(q.device))
+        nat.check("mixfp4_fp8_dequant", st)
+    return out
+
+
+@torch.no_grad()
+def fp8_linear(x: torch.Tensor | FP8Activations, weight: FP8Weight, *, bias: torch.Tensor | None = None,
+               out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """y = x @ W^T (+ bias) on block-scaled FP8 operands.  x: a dense tensor [..., K] (bf16, f16 or fp32), quantized within
+    the call, or what `quantize_fp8_activations` made of one.  out_dtype: bf16, f16 or fp32 (default: x's dtype).  A product
+    whose device-side waits run out reports through `gemm_status()`, like the other GEMMs."""
+    k, n, device = weight.k, weight.n, weight.device
+    quantized = isinstance(x, FP8Activations)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _OUT_DTYPES:
+        raise TypeError("out_dtype must be bfloat16, float16 or float32")
+    if x.shape[-1] != k:
+        raise ValueError(f"x has K={x.shape[-1]}, the weight K={k}")
+    if x.device != device:
+        raise ValueError(f"x is on {x.device}, the weight on {device}")
+    nat.require_cuda(weight.codes, "the weight")
+    lead = x.shape[:-1]
+    x2 = x.codes if quantized else _rows(x, "x")
+    m = x2.shape[0]
+    y = torch.empty((m, n), dtype=out_dtype, device=device)
+    if m:
+        lib = nat.lib()
+        w = weight.codes.data_ptr(), weight.codes.stride(0), weight.scales.data_ptr()
+        with nat.on_device(device):
+            stream = nat.stream_ptr(device)
+            if quantized:
+                st = lib.mixfp4_fp8_gemm(x2.data_ptr(), x2.stride(0), x.scales.data_ptr(), x.scales.stride(1), *w,
+                                         m, n, k, y.data_ptr(), nat.DTYPE_CODE[out_dtype], n, _status_word(device).data_ptr(),
+                                         stream)
+                nat.check("mixfp4_fp8_gemm", st)
+            else:
+                nbytes = lib.mixfp4_fp8_workspace_bytes(m, k)
+                work = torch.empty(nbytes, dtype=torch.uint8, device=device)      # a captured graph's own
+                st = lib.mixfp4_fp8_linear(x2.data_ptr(), nat.DTYPE_CODE[x2.dtype], m, x2.stride(0), *w, n, k,
+                                           y.data_ptr(), nat.DTYPE_CODE[out_dtype], n, work.data_ptr(), nbytes,
+                                           _status_word(device).data_ptr(), stream)
+                nat.check("mixfp4_fp8_linear", st)
+    if bias is not None:
+        y += bias.to(y.dtype)
+    return y if len(lead) == 1 else y.reshape(*lead, n)
+
+
+class FP8Linear(nn.Module):
+    """nn.Linear whose weight is held in block-scaled FP8; inference only, like MixFP4Linear."""
+
+    def __init__(self, weight: FP8Weight, bias: torch.Tensor | None = None):
+        super().__init__()
+        self.in_features, self.out_features = weight.k, weight.n
+        self.register_buffer("codes", weight.codes)
+        self.register_buffer("scales", weight.scales)
+        self.bias = None if bias is None else nn.Parameter(bias.detach().clone(), requires_grad=False)
+
+    def _apply(self, fn, recurse=True):
+        """Moves between devices; a change of type (`model.half()`) reaches the bias alone: codes and scales are the format's."""
+        held = self.weight_fp8
+        super()._apply(fn, recurse)
+        moved = held if self.codes.device == held.device else held.to(self.codes.device)
+        self.codes, self.scales = moved.codes, moved.scales
+        return self
+
+    @property
+    def weight_fp8(self) -> FP8Weight:
+        return FP8Weight(self.codes, self.scales)
+
+    @classmethod
+    @torch.no_grad()
+    def from_linear(cls, linear: nn.Linear, *, device=None) -> "FP8Linear":
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+        w = linear.weight.detach().to(device)
+        bias = None if linear.bias is None else linear.bias.detach().to(device)
+        return cls(quantize_fp8_weight(w if w.dtype in nat.DTYPE_CODE else w.to(torch.bfloat16)), bias)
+
+    def forward(self, x: torch.Tensor | FP8Activations, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+        return fp8_linear(x, self.weight_fp8, bias=self.bias, out_dtype=out_dtype)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}"

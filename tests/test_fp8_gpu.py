@@ -1,0 +1,238 @@
+"""The block-scaled FP8 quantizers and product against plain arithmetic in 64 bits."""
+
+import pytest
+import torch
+
+import mixfp4_b200 as mx
+from mixfp4_b200 import _native as nat
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+SUBNORMAL = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}
+
+
+def _e4m3(v):
+    """Nearest E4M3 value of doubles, ties to the even mantissa."""
+    _, e = torch.frexp(v)
+    step = torch.ldexp(torch.ones_like(v), (e - 1).clamp(min=-6) - 3)
+    return (torch.round(v / step) * step).clamp(-448, 448)
+
+
+def _reference(x, rows):
+    """(code values, scales) as doubles, block by block."""
+    r, k = x.shape
+    values, scales = torch.zeros((r, k), dtype=torch.float64), torch.zeros((-(-r // rows), -(-k // 128)), dtype=torch.float64)
+    x = x.double().cpu()
+    for i in range(scales.shape[0]):
+        for b in range(scales.shape[1]):
+            part = x[i * rows: (i + 1) * rows, 128 * b: 128 * b + 128]
+            s = (part.abs().max() / 448).float().double()
+            s = s if s != 0 else torch.ones((), dtype=torch.float64)
+            scales[i, b] = s
+            values[i * rows: (i + 1) * rows, 128 * b: 128 * b + 128] = _e4m3((part / s).float().double())
+    return values, scales
+
+
+def _expand(values, scales, rows):
+    s = scales.double().repeat_interleave(rows, 0)[: values.shape[0]].repeat_interleave(128, 1)[:, : values.shape[1]]
+    return values.double() * s
+
+
+def _data(r, k, dtype, seed, spread=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((r, k), generator=g)
+    if spread:
+        x *= torch.exp(torch.randn((r, 1), generator=g)) * torch.exp(2 * torch.randn((1, k), generator=g))
+    return x.to(dtype).cuda()
+
+
+def _check_product(y, a, b, out_dtype):
+    """Sums of 128 products by the tensor core, each addition off by a whole step at most (it may cut instead of round);
+    the scale products, the additions of the blocks and the result are rounded."""
+    ref = a.double() @ b.double().T
+    room = a.double().abs() @ b.double().abs().T
+    blocks = -(-a.shape[1] // 128)
+    limit = (2 * 128 + blocks + 4) * 2.0 ** -24 * room + HALF_STEP[out_dtype] * ref.abs() + SUBNORMAL[out_dtype]
+    over = ref.abs() > torch.finfo(out_dtype).max             # what the type cannot hold is an infinity in it
+    assert (y[over].isinf() & (y[over] > 0).eq(ref[over] > 0)).all()
+    worst = ((y.double() - ref).abs() / limit)[~over].max().item()
+    assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 128), (3, 127), (5, 129), (128, 256), (130, 1500), (2, 4096)])
+def test_quantizers_match_the_definition(dtype, rows, k):
+    x = _data(rows, k, dtype, 7 * rows + k)
+    q = mx.quantize_fp8_activations(x)
+    values, scales = _reference(x, 1)
+    assert torch.equal(q.codes.double().cpu(), values) and torch.equal(q.scales.double().cpu(), scales)
+    w = mx.quantize_fp8_weight(x)
+    values, scales = _reference(x, 128)
+    assert torch.equal(w.codes.double().cpu(), values) and torch.equal(w.scales.double().cpu(), scales)
+    for what, per in ((q, 1), (w, 128)):
+        for out in (torch.bfloat16, torch.float16, torch.float32):
+            dense = mx.dequantize_fp8(what, out)
+            plain = (what.codes.float() * _expand(torch.ones(rows, k, device="cuda"), what.scales, per).float()).to(out)
+            assert torch.equal(dense, plain)
+
+
+def test_quantizer_block_extremes():
+    x = torch.zeros((6, 384), device="cuda")
+    x[1, 5] = 1e-45                                          # the scale would be zero
+    x[2, :128] = torch.linspace(-1e-38, 1e-38, 128)          # a subnormal scale
+    x[3, 130] = 3.0e38
+    x[4, 0], x[4, 300] = float("inf"), float("nan")
+    x[5] = torch.arange(384) * 2.0 ** -12
+    q = mx.quantize_fp8_activations(x)
+    assert (q.scales[:2] == 1).all() and (q.codes[:2].float() == 0).all()
+    values, scales = _reference(x[[2, 3, 5]], 1)
+    assert torch.equal(q.codes.double().cpu()[[2, 3, 5]], values) and torch.equal(q.scales.double().cpu()[[2, 3, 5]], scales)
+    assert q.scales[4, 0].isinf() and q.scales[4, 1] == 1 and q.scales[4, 2].isnan()
+    w = mx.quantize_fp8_weight(torch.ones((4, 384), device="cuda"))
+    y = mx.fp8_linear(x, w)
+    assert y[4].isnan().all() and y[[0, 1, 2, 3, 5]].isfinite().all()
+
+
+def test_quantizer_takes_strides_and_leaves_other_memory():
+    base = torch.full((40, 700), 5.0, device="cuda")
+    for view in (base[3:20, 1:300], base[::2, 100:400], base[:, 7:8], base.t()[10:20, :30]):
+        a, b = mx.quantize_fp8_activations(view), mx.quantize_fp8_activations(view.contiguous())
+        assert torch.equal(a.codes.float(), b.codes.float()) and torch.equal(a.scales, b.scales)
+    x = _data(130, 200, torch.bfloat16, 3)
+    codes = torch.full((132, 256), 0x55, dtype=torch.uint8, device="cuda")
+    scales = torch.full((2, 256), -7.0, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert nat.lib().mixfp4_fp8_quantize_rows(x.data_ptr(), nat.BF16, 130, 200, 200, codes.data_ptr(), 256, scales.data_ptr(), 256, stream) == 0
+    assert (codes[130:] == 0x55).all() and (codes[:130, 200:] == 0).all() and (scales[:, 130:] == -7).all() and (scales[:, :130] > 0).all()
+
+
+SHAPES = [(1, 1, 1), (1, 128, 128), (1, 1024, 4096), (2, 130, 129), (7, 200, 1000), (16, 4096, 512), (17, 128, 14336), (32, 257, 300),
+          (33, 1000, 2048), (64, 300, 4224), (65, 128, 128), (100, 384, 700), (129, 1000, 1500), (333, 515, 260), (777, 1024, 1024),
+          (1024, 2048, 640), (2500, 2304, 384)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_linear_against_64_bits(m, n, k):
+    x, w = _data(m, k, torch.bfloat16, m + k), _data(n, k, torch.bfloat16, n + k + 1)
+    weight, q = mx.quantize_fp8_weight(w), mx.quantize_fp8_activations(x)
+    a, b = _expand(q.codes, q.scales, 1), _expand(weight.codes, weight.scales, 128)
+    for out in (torch.bfloat16, torch.float32) + ((torch.float16,) if m == 7 else ()):
+        y = mx.fp8_linear(x, weight, out_dtype=out)
+        assert y.shape == (m, n) and y.dtype == out
+        _check_product(y, a, b, out)
+        assert torch.equal(y, mx.fp8_linear(q, weight, out_dtype=out)), "quantized within the call or before it"
+    assert mx.gemm_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_linear_input_types_and_leading_dimensions(dtype):
+    x, w = _data(30, 500, dtype, 1), _data(70, 500, torch.float32, 2)
+    weight = mx.quantize_fp8_weight(w)
+    q = mx.quantize_fp8_activations(x)
+    y = mx.fp8_linear(x.reshape(2, 3, 5, 500), weight)
+    assert y.shape == (2, 3, 5, 70) and y.dtype == dtype
+    _check_product(y.reshape(30, 70), _expand(q.codes, q.scales, 1), _expand(weight.codes, weight.scales, 128), dtype)
+    bias = torch.randn(70, device="cuda")
+    assert torch.equal(mx.fp8_linear(x, weight, bias=bias), mx.fp8_linear(x, weight) + bias.to(dtype))
+    assert torch.equal(mx.fp8_linear(x[0], weight), mx.fp8_linear(x[:1], weight)[0])
+    assert mx.fp8_linear(x[:0], weight).shape == (0, 70)
+    wide = torch.zeros((30, 777), dtype=dtype, device="cuda")
+    wide[:, 5:505] = x
+    assert torch.equal(mx.fp8_linear(wide[:, 5:505], weight), mx.fp8_linear(x, weight))
+    assert torch.equal(mx.fp8_linear(x[:1].expand(4, 500), weight), mx.fp8_linear(x[:1], weight).expand(4, 70))
+
+
+def test_linear_writes_nothing_but_its_rows():
+    x, w = _data(70, 256, torch.bfloat16, 1), _data(130, 256, torch.bfloat16, 2)
+    weight, q = mx.quantize_fp8_weight(w), mx.quantize_fp8_activations(x)
+    for m in (3, 70):
+        for ld in (130, 133, 160):
+            y = torch.full((m + 2, ld), -9.0, dtype=torch.bfloat16, device="cuda")
+            part = mx.quantize_fp8_activations(x[:m])
+            rc = nat.lib().mixfp4_fp8_gemm(part.codes.data_ptr(), part.codes.stride(0), part.scales.data_ptr(), part.scales.stride(1),
+                                           weight.codes.data_ptr(), weight.codes.stride(0), weight.scales.data_ptr(), m, 130, 256,
+                                           y.data_ptr(), nat.BF16, ld, None, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            assert torch.equal(y[:m, :130], mx.fp8_linear(part, weight)) and (y[m:] == -9).all() and (y[:m, 130:] == -9).all()
+
+
+def test_rows_do_not_depend_on_the_batch():
+    """Within one arrangement a row's result is the same bits whatever stands beside it, and repeats of a call agree."""
+    x, w = _data(64, 4096, torch.bfloat16, 5), _data(512, 4096, torch.bfloat16, 6)
+    weight = mx.quantize_fp8_weight(w)
+    y = mx.fp8_linear(x, weight, out_dtype=torch.float32)
+    for _ in range(3):
+        assert torch.equal(y, mx.fp8_linear(x, weight, out_dtype=torch.float32))
+    perm = torch.randperm(64, device="cuda")
+    assert torch.equal(mx.fp8_linear(x[perm], weight, out_dtype=torch.float32), y[perm])
+
+
+def test_imported_tensors():
+    w = _data(200, 300, torch.bfloat16, 9)
+    weight = mx.quantize_fp8_weight(w)
+    x = _data(20, 300, torch.bfloat16, 10)
+    y = mx.fp8_linear(x, weight)
+    dense = weight.codes.contiguous()                        # 300-byte rows: copied into aligned ones
+    again = mx.FP8Weight.from_tensors(dense.view(torch.uint8), weight.scales.clone())
+    assert again.codes.stride(0) % 16 == 0 and torch.equal(mx.fp8_linear(x, again), y)
+    q = mx.quantize_fp8_activations(x)
+    assert torch.equal(mx.fp8_linear(mx.FP8Activations.from_tensors(q.codes.contiguous(), q.scales.contiguous()), weight), y)
+    assert torch.equal(q.dequantize(torch.float32), mx.dequantize_fp8(q, torch.float32))
+
+
+def test_captured_and_on_another_stream():
+    x, w = _data(5, 1024, torch.bfloat16, 1), _data(384, 1024, torch.bfloat16, 2)
+    weight = mx.quantize_fp8_weight(w)
+    want = mx.fp8_linear(x, weight)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, slots = [], [torch.zeros_like(x), torch.zeros_like(x)]
+    with torch.cuda.stream(side):
+        assert torch.equal(mx.fp8_linear(x, weight), want)
+        torch.cuda.synchronize()
+        for slot in slots:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                y = mx.fp8_linear(slot, weight)
+            graphs.append((g, y))
+    slots[0].copy_(x)
+    slots[1].copy_(2 * x)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):                                      # two graphs of one stream's capture, at once
+        for (g, _), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[0][1], want) and torch.equal(graphs[1][1], 2 * want)
+
+
+def test_module_keeps_its_format():
+    dense = torch.nn.Linear(300, 200, bias=True, device="cuda", dtype=torch.bfloat16)
+    layer = mx.FP8Linear.from_linear(dense)
+    x = _data(9, 300, torch.bfloat16, 4)
+    y = layer(x)
+    assert torch.equal(y, mx.fp8_linear(x, mx.quantize_fp8_weight(dense.weight), bias=dense.bias))
+    layer = layer.half().cpu().cuda().bfloat16()
+    assert layer.codes.dtype == torch.float8_e4m3fn and layer.scales.dtype == torch.float32
+    assert torch.equal(layer(x), mx.fp8_linear(x, mx.quantize_fp8_weight(dense.weight), bias=layer.bias))
+    other = mx.FP8Linear.from_linear(torch.nn.Linear(300, 200, device="cuda", dtype=torch.bfloat16))
+    other.load_state_dict(layer.state_dict())
+    assert torch.equal(other(x), layer(x))
+
+
+def test_refusals():
+    x, weight = _data(4, 256, torch.bfloat16, 1), mx.quantize_fp8_weight(_data(64, 256, torch.bfloat16, 2))
+    with pytest.raises(ValueError):
+        mx.fp8_linear(x[:, :128], weight)
+    with pytest.raises(TypeError):
+        mx.fp8_linear(x, weight, out_dtype=torch.float64)
+    with pytest.raises(TypeError):
+        mx.fp8_linear(x.double(), weight, out_dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        mx.fp8_linear(x.cpu(), weight)
+    with pytest.raises(ValueError):
+        mx.FP8Weight.from_tensors(weight.codes, weight.scales[:, :1])
+    with pytest.raises(TypeError):
+        mx.FP8Weight.from_tensors(weight.codes, weight.scales.half())

@@ -1,0 +1,177 @@
+"""sample_logits against a plain implementation in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+import mixfp4_b200 as mx
+
+pytestmark = pytest.mark.gpu
+
+INF = math.inf
+
+
+def _reference(x, u, t, k, p, f):
+    """One row, doubles: (token, log probability)."""
+    x = [(-INF if math.isnan(v) else v) for v in x]
+    top = max(x)
+    if top == -INF:
+        return -1, -INF
+    order = sorted(range(len(x)), key=lambda i: (-x[i], i))
+    if not t > 0:
+        return order[0], 0.0
+    w = [1.0 if v == top else math.exp((v - top) / t) if top != INF else 0.0 for v in x]
+    if k > 0:
+        order = order[:k]
+    if p < 1:
+        goal, run, n = p * math.fsum(w[i] for i in order), 0.0, 0
+        while n == 0 or run < goal:
+            run += w[order[n]]
+            n += 1
+            if n == len(order):
+                break
+        order = order[:n]
+    kept = sorted(i for i in order if w[i] >= min(f, 1.0) and w[i] > 0)
+    total = math.fsum(w[i] for i in kept)
+    run = 0.0
+    for i in kept:
+        run += w[i]
+        if run > u * total:
+            break
+    return i, math.log(w[i] / total)
+
+
+def _check(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    token, logprob = mx.sample_logits(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, return_logprob=True)
+    rows = logits.shape[0]
+    each = lambda v: v.double().tolist() if isinstance(v, torch.Tensor) else [v] * rows
+    t, k, p, f = each(temperature), each(top_k), each(top_p), each(min_p)
+    x = logits.double().cpu().tolist()
+    for r, (a, b, v) in enumerate(zip(token.tolist(), logprob.tolist(), u.double().tolist())):
+        want, lp = _reference(x[r], v, t[r], int(k[r]), p[r], f[r])
+        assert a == want, (r, a, want)
+        # the log of a share: weights and sums are held to 2^-44 of the largest, the result is rounded to 24 bits
+        assert b == lp or abs(b - lp) <= 2.0 ** -24 * abs(lp) + 1e-9, (r, b, lp)
+
+
+def _logits(rows, vocab, dtype, seed, scale=3.0):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn((rows, vocab), generator=g)).to(dtype).cuda(), torch.rand(rows, generator=g).cuda()
+
+
+SETTINGS = [dict(), dict(temperature=0.0), dict(temperature=0.6, top_k=1), dict(top_k=50, top_p=0.9), dict(temperature=1.4, top_p=0.5),
+            dict(min_p=0.1), dict(temperature=0.8, top_k=20, top_p=0.95, min_p=0.02), dict(top_p=0.0), dict(top_k=1000, top_p=0.999),
+            dict(min_p=1.0), dict(temperature=0.05), dict(temperature=50.0, top_p=0.99)]
+
+
+@pytest.mark.parametrize("settings", SETTINGS, ids=lambda s: "-".join(f"{k}{v}" for k, v in s.items()) or "plain")
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_against_64_bits(dtype, settings):
+    for rows, vocab, seed in ((3, 1, 1), (5, 17, 2), (40, 1001, 3), (2, 40003, 4)):
+        _check(*_logits(rows, vocab, dtype, seed), **settings)
+
+
+@pytest.mark.parametrize("rows", [1, 8, 30, 100])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_every_split_of_a_row(rows, dtype):
+    """Rows of 1 to 8 CTAs; a vocabulary past what shared memory holds of fp32 rows in the last."""
+    _check(*_logits(rows, 9000, dtype, rows), temperature=0.9, top_k=300, top_p=0.97)
+    if rows == 1:
+        _check(*_logits(1, 500000, dtype, 9), temperature=0.9, top_p=0.9)
+
+
+def test_equal_values_are_counted_off_by_index():
+    x = torch.zeros((64, 5003), device="cuda")
+    u = ((torch.arange(64, dtype=torch.float32) + 0.5) / 64).cuda()
+    for settings in (dict(), dict(top_k=1), dict(top_k=37), dict(top_k=4999, top_p=0.5), dict(top_p=0.25), dict(top_p=0.9), dict(top_k=5003)):
+        _check(x, u, **settings)
+    x[:, 100:4000] = 2.0
+    for settings in (dict(top_k=3000), dict(top_k=4500), dict(top_p=0.5), dict(top_p=0.99), dict(top_k=4200, top_p=0.999)):
+        _check(x, u, **settings)
+    few = torch.randint(-3, 4, (64, 3001), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    for settings in (dict(top_k=700), dict(top_p=0.6), dict(top_k=300, top_p=0.9), dict(temperature=0.0)):
+        _check(few, u, **settings)
+    zeros = torch.where(few == 0, -few, few)                 # zeros of both signs are one value
+    zeros[:, ::2] = few[:, ::2]
+    _check(zeros, u, top_k=1500)
+
+
+def test_masked_rows_and_values_that_are_not_finite():
+    x, u = _logits(8, 3000, torch.float32, 5)
+    lowest = torch.finfo(torch.float32).min
+    x[0] = -INF
+    x[1] = math.nan
+    x[2, :-1] = -INF
+    x[3, 1:] = lowest
+    x[4] = lowest
+    x[5, [7, 2999]] = INF
+    x[6, ::2] = math.nan
+    x[7, 100:] = -INF
+    for settings in (dict(), dict(temperature=0.0), dict(top_k=5), dict(top_p=0.9), dict(top_k=50, top_p=0.5, min_p=0.05)):
+        _check(x, u, **settings)
+    token, logprob = mx.sample_logits(x, u, return_logprob=True)
+    assert token[:3].tolist() == [-1, -1, 2999] and logprob[:3].tolist() == [-INF, -INF, 0.0]
+
+
+def test_a_setting_for_each_row():
+    x, u = _logits(50, 2000, torch.bfloat16, 8)
+    pick = lambda values, dtype: torch.tensor([values[i % len(values)] for i in range(50)], dtype=dtype, device="cuda")
+    _check(x, u, temperature=pick([0.0, 0.7, 1.0, 1.5, 0.3], torch.float32), top_k=pick([0, 5, 100, -1], torch.int32),
+           top_p=pick([1.0, 0.9, 0.5], torch.float32), min_p=pick([0.0, 0.0, 0.05, 0.2, 0.0, 0.0, 1.0], torch.float32))
+
+
+def test_ends_of_the_random_numbers():
+    x, _ = _logits(6, 700, torch.float32, 3)
+    u = torch.tensor([0.0, 1.0 - 2.0 ** -24, 1.0, 2.0, -1.0, math.nan], device="cuda")
+    token = mx.sample_logits(x, u, top_k=9).tolist()
+    kept = x.topk(9, dim=1).indices.sort(dim=1).values.tolist()
+    assert token == [kept[0][0], kept[1][-1], kept[2][-1], kept[3][-1], kept[4][0], kept[5][0]]
+
+
+def test_strides_shapes_streams_and_capture():
+    x, u = _logits(6, 1500, torch.bfloat16, 4)
+    want = mx.sample_logits(x, u, top_p=0.9)
+    wide = torch.full((6, 1777), 50.0, dtype=torch.bfloat16, device="cuda")
+    wide[:, 3:1503] = x
+    assert torch.equal(mx.sample_logits(wide[:, 3:1503], u, top_p=0.9), want)
+    assert torch.equal(mx.sample_logits(x.t().contiguous().t(), u, top_p=0.9), want)
+    assert torch.equal(mx.sample_logits(x.reshape(2, 3, 1500), u.reshape(2, 3), top_p=0.9), want.reshape(2, 3))
+    assert mx.sample_logits(x[0], u[0], top_p=0.9).shape == () and mx.sample_logits(x[:0], u[:0]).shape == (0,)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(g, stream=side):
+            token = mx.sample_logits(x, u, top_p=0.9)
+    x.copy_(x.flip(0))
+    u.copy_(u.flip(0))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(token, want.flip(0))
+
+
+def test_head_and_sampling_together():
+    """A step's end as the decoder runs it: head product in FP8, then a token; the token follows from the logits."""
+    g = torch.Generator().manual_seed(2)
+    head = mx.quantize_fp8_weight((0.05 * torch.randn((5000, 512), generator=g)).to(torch.bfloat16).cuda())
+    h, u = torch.randn((12, 512), generator=g).to(torch.bfloat16).cuda(), torch.rand(12, generator=g).cuda()
+    _check(mx.fp8_linear(h, head), u, temperature=0.8, top_k=40, top_p=0.95)
+
+
+def test_refusals():
+    x, u = _logits(4, 100, torch.float32, 1)
+    for bad in (dict(temperature=-1.0), dict(top_p=1.5), dict(min_p=-0.1), dict(top_p=torch.ones(3, device="cuda"))):
+        with pytest.raises(ValueError):
+            mx.sample_logits(x, u, **bad)
+    for bad in (dict(top_k=2.5), dict(top_k=torch.ones(4, device="cuda")), dict(temperature="1")):
+        with pytest.raises(TypeError):
+            mx.sample_logits(x, u, **bad)
+    with pytest.raises(ValueError):
+        mx.sample_logits(x, u[:3])
+    with pytest.raises(TypeError):
+        mx.sample_logits(x, u.double())
+    with pytest.raises(TypeError):
+        mx.sample_logits(x.double(), u)
+    with pytest.raises(mx._native.MixFP4Error):
+        mx.sample_logits(torch.zeros((1, 600000), device="cuda"), u[:1])
