@@ -8,13 +8,20 @@
 // histograms: 1024 bins of equal width over the logits that have a weight at all, then 1024 bins of the keys (a monotone
 // integer of the value) in the bin that the cut falls in, until that bin is one value; equal values are counted off by
 // index.  Every CTA adds the cluster's histograms up for itself: one cluster barrier a step, none to hand a result round.
+// Where the first histogram leaves at most 256 candidates for a top-k (the usual settings), one CTA takes them all and
+// compares each with each.
 //
 // Sums.  The set of kept tokens and the token itself hang on comparisons of sums over the vocabulary, so weights are
 // integers: W = round(2^44 w), w in double precision.  Integer sums do not depend on their order, so neither do the
 // results, and 2^19 of them fit 63 bits.  A weight below 2^-45 of the largest counts as none.  Shared memory adds 32-bit
-// words only, so a bin's sum is kept as three limbs of 16 bits, which 65536 values cannot overflow: the largest slice of a CTA.
+// words only, so a bin's sum is two words, and whoever overflows the low one adds the carry to the high one: one addition
+// for all but the largest few thousandths of the weights.
+//
+// What bounds it: a row of a small batch takes a dozen dependent steps (passes over shared memory, cluster barriers), and
+// code that runs once or twice: instruction fetch counts, so every pass has one copy (86 KB of unrolled passes took 70 us for
+// one row of 128256 logits with top-k and top-p, a third of that code 39 us).  Large batches: the fp64 operations of the weights.
 
-#include <mutex>
+#include <float.h>
 
 #include "common.cuh"
 
@@ -25,7 +32,9 @@ constexpr int kSampleThreads = 1024, kSampleWarps = kSampleThreads / 32, kBins =
 static_assert(kBins == kSampleThreads, "a thread owns a bin");
 constexpr int kMaxRanks = 8;
 constexpr int64_t kMaxSlice = 65536, kMaxVocab = kMaxRanks * kMaxSlice - 128;
+constexpr int kOneLog = 44;
 constexpr double kOne = 17592186044416.0;                // 2^44
+constexpr int kSteps = 64;                               // of an octave, in the table of the exponential
 constexpr float kSpan = 31.5f;                           // weights vanish at 45 ln 2 = 31.2
 constexpr float kNegInf = -__builtin_huge_valf();
 
@@ -73,15 +82,18 @@ struct Slots {
     uint32_t count[kMaxRanks];
     u64 mass[kMaxRanks];
 };
+constexpr uint32_t kFew = 256;
 struct Shared {
-    uint4 hist[2][kBins];                                // per bin: count, three limbs of the weights' sum
+    u64 mass[2][kBins];                                  // per bin, as two words
+    uint32_t count[2][kBins];
+    double octave[kSteps];                               // 2^(j / kSteps)
+    u64 few[kFew], few_weight[kFew];                     // candidates: key, then the index turned round
     Slots slots[2];
     u64 warp_mass[kSampleWarps];
     uint32_t warp_count[kSampleWarps];
     float warp_max[kSampleWarps];
-    u64 found_mass;
-    uint32_t found_count, found_bin, found_size;
-    u64 total_mass;
+    u64 found_before;
+    uint32_t found_bin, found_size, few_count;
 };
 
 __device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -90,9 +102,14 @@ __device__ __forceinline__ uint32_t of_rank(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ uint4 ld_rank(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+__device__ __forceinline__ uint32_t ld_rank32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ u64 ld_rank64(uint32_t addr) {
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ void st_rank32(uint32_t addr, uint32_t v) {
@@ -101,15 +118,42 @@ __device__ __forceinline__ void st_rank32(uint32_t addr, uint32_t v) {
 __device__ __forceinline__ void st_rank64(uint32_t addr, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
+__device__ __forceinline__ uint32_t add_rank32(uint32_t addr, uint32_t v) {
+    uint32_t was;
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(was) : "r"(addr), "r"(v) : "memory");
+    return was;
+}
 __device__ __forceinline__ void meet(int ranks) {        // all threads of the cluster; writes before are seen after
     if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     else __syncthreads();
 }
-
-// A prefix of the sorted row: everything with a larger key than `key`, and the first `ties` of those equal to it.
+// Sum over this lane and those before it.
+__device__ __noinline__ u64 add_up(u64 v) {
+#pragma unroll 1
+    for (int d = 1; d < 32; d *= 2) {
+        const u64 o = __shfl_up_sync(0xffffffffu, v, d);
+        if ((int)(threadIdx.x & 31) >= d) v += o;
+    }
+    return v;
+}
+// A prefix of the sorted row: everything above `value`, and the first `ties` of those equal to it.
 struct Cut {
-    uint32_t key, ties, equal;                           // equal: how many there are
+    float value;
+    uint32_t ties, equal;                                // equal: how many there are
 };
+
+// Out of line: once a row, and long.
+__device__ __noinline__ double log_of(u64 total) { return log((double)total / kOne); }
+__device__ __noinline__ double octave_step(int j) { return exp2((double)j / kSteps); }
+// 16 bytes at a row's end: the elements [0, n) of it from index i, -inf around them.
+template <typename T>
+__device__ __noinline__ uint4 fetch_end(const T* row, int i, int n) {
+    uint4 u;
+    T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int j = 0; j < 16 / (int)sizeof(T); ++j) e[j] = i + j >= 0 && i + j < n ? row[i + j] : Elem<T>::round(kNegInf);
+    return u;
+}
 
 template <typename T, bool kResident>
 struct Sampler {
@@ -118,149 +162,140 @@ struct Sampler {
     Shared& s;
     uint4* held;                                         // kResident: the slice's granules
     const T* row;
-    int skew, granules, g0, g1;                          // granules of the row; this warp's
-    int warp, lane, rank, turn, hist_turn;
-    float largest;
-    double inv_t;
+    int skew, first, c0, c1;                             // first granule of this CTA; this warp's quads
+    int warp, lane, rank, hist_turn;
+    float largest, floor_x;                              // below floor_x nothing has a weight
+    double top;                                          // the largest, if that is finite
+    double inv_t, steps_t;                               // 1 / T, kSteps log2(e) / T
     float bin_scale;
 
-    // Element j of granule g has index g * kPer + j - skew: granules start on 16-byte boundaries, the row need not.
-    __device__ void fetch(int g, float (&v)[kPer]) const {
-        const int first = g * kPer - skew;
-        if (first >= 0 && first + kPer <= a.vocab) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + first));
-            const T* e = reinterpret_cast<const T*>(&u);
+    // Granule g holds the indices g * kPer - skew ..: granules start on 16-byte boundaries, the row need not.  NaN and what
+    // lies outside the row count as -inf (the larger of NaN and a number is the number).
+    __device__ uint4 fetch(int g) const {
+        const int i = g * kPer - skew;
+        uint4 u = i >= 0 && i + kPer <= a.vocab ? __ldg(reinterpret_cast<const uint4*>(row + i)) : fetch_end(row, i, a.vocab);
+        if constexpr (sizeof(T) == 4) {
+            float* e = reinterpret_cast<float*>(&u);
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) v[j] = Elem<T>::load(e + j);
+            for (int j = 0; j < kPer; ++j) e[j] = fmaxf(e[j], kNegInf);
         } else {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) v[j] = first + j >= 0 && first + j < a.vocab ? Elem<T>::load(row + first + j) : kNegInf;
+            auto clean = [](uint32_t w) {
+                if constexpr (Elem<T>::kDtype == MIXFP4_BF16) {
+                    const __nv_bfloat162 c = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&w), __float2bfloat162_rn(kNegInf));
+                    return *reinterpret_cast<const uint32_t*>(&c);
+                } else {
+                    const __half2 c = __hmax2(*reinterpret_cast<__half2*>(&w), __float2half2_rn(kNegInf));
+                    return *reinterpret_cast<const uint32_t*>(&c);
+                }
+            };
+            u = make_uint4(clean(u.x), clean(u.y), clean(u.z), clean(u.w));
         }
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-            if (isnan(v[j])) v[j] = kNegInf;
+        return u;
     }
-    __device__ void get(int g, int base, float (&v)[kPer]) const {
+    // Quad c, four elements from index 4 c - skew.  A warp's pass takes a quad a lane at a time: code for four elements is short,
+    // and four weights at once hide the latency of their operations.
+    __device__ void get(int c, float (&x)[4]) const {
+        constexpr int kQuads = kPer / 4;
+        const T* e;
+        uint4 u;
         if constexpr (kResident) {
-            const uint4 u = held[g - base];
-            const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) v[j] = Elem<T>::load(e + j);
+            if constexpr (sizeof(T) == 4) {
+                u = held[c - first];
+            } else {
+                const uint2 half = reinterpret_cast<const uint2*>(held)[c - first * kQuads];
+                u.x = half.x; u.y = half.y;
+            }
+            e = reinterpret_cast<const T*>(&u);
         } else {
-            fetch(g, v);
+            u = fetch(c / kQuads);
+            if (kQuads > 1 && c % kQuads) { u.x = u.z; u.y = u.w; }
+            e = reinterpret_cast<const T*>(&u);
         }
-    }
-    int base;                                            // first granule of this CTA
-
-    // f(value, index) for this warp's elements in the order of a granule's elements; lanes take granules in turn.
-    template <typename F>
-    __device__ void each(F&& f) const {
-        for (int g = g0 + lane; g < g1; g += 32) {
-            float v[kPer];
-            get(g, base, v);
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) f(v[j], g * kPer + j - skew);
-        }
+        for (int j = 0; j < 4; ++j) x[j] = Elem<T>::load(e + j);
     }
 
-    __device__ double weight(float x) const { return x == largest ? 1.0 : exp(((double)x - (double)largest) * inv_t); }
-    __device__ u64 fixed(float x) const { return (u64)__double2ll_rn(weight(x) * kOne); }
-    // Bin of equal width, rising as the value falls (rounded operations are monotone); kBins and more: no weight.
-    __device__ uint32_t linear(float x) const {
-        if (x == kNegInf) return kBins;
-        const float d = x == largest ? 0.0f : largest - x;
-        return (uint32_t)fminf(d * bin_scale, (float)kBins);
+    // 2^44 w for x >= floor_x: y = log2(w) in steps of an octave, rounded to a whole step by an addition that leaves no fraction
+    // bits; the rest of at most half a step by its series (the next term is 4e-14), the step from the table, the octave into
+    // the exponent.  To the nearest integer: below 2^52, an addition of 2^52 leaves it in the low bits.
+    __device__ u64 weight(float x) const {
+        const double y = ((double)fminf(x, FLT_MAX) - top) * steps_t;
+        const double shifted = y + 0x1.8p52;
+        const int i = __double2loint(shifted);
+        const double r = y - (shifted - 0x1.8p52);
+        constexpr double c = 0.69314718055994530942 / kSteps;
+        double e = c * c * c * c / 24;
+        e = fma(e, r, c * c * c / 6);
+        e = fma(e, r, c * c / 2);
+        e = fma(e, r, c);
+        e = fma(e, r, 1.0) * s.octave[i & (kSteps - 1)];
+        static_assert(kSteps == 1 << 6, "the shift below");
+        e = __hiloint2double(__double2hiint(e) + (((i >> 6) + kOneLog) << 20), __double2loint(e));
+        return (u64)__double_as_longlong(e + 0x1p52) & 0xfffffffffffffull;
     }
+    // Bin of equal width, rising as the value falls (rounded operations are monotone).  The conversion takes what is too
+    // large to its own largest value, and infinity less infinity, a NaN, to 0.
+    __device__ uint32_t linear(float x) const { return min(__float2uint_rz((largest - x) * bin_scale), (uint32_t)kBins - 1); }
 
     __device__ void clear(int which) {
-        s.hist[which][threadIdx.x] = make_uint4(0, 0, 0, 0);
+        s.count[which][threadIdx.x] = 0;
+        s.mass[which][threadIdx.x] = 0;
     }
-    __device__ void put(int which, uint32_t bin, bool masses, float x) {
-        uint32_t* h = reinterpret_cast<uint32_t*>(&s.hist[which][bin]);
-        atomicAdd(h, 1u);
-        if (masses) {
-            const u64 w = fixed(x);
-            atomicAdd(h + 1, (uint32_t)(w & 0xffffu));
-            atomicAdd(h + 2, (uint32_t)(w >> 16) & 0xffffu);
-            atomicAdd(h + 3, (uint32_t)(w >> 32));
+    __device__ void put(uint32_t bin, bool counted, u64 w) {
+        if (counted) atomicAdd(&s.count[hist_turn][bin], 1u);
+        if (w) {
+            uint32_t* words = reinterpret_cast<uint32_t*>(&s.mass[hist_turn][bin]);
+            const uint32_t low = (uint32_t)w, was = atomicAdd(words, low);
+            const uint32_t high = (uint32_t)(w >> 32) + (was + low < was);
+            if (high) atomicAdd(words + 1, high);
         }
     }
-    // The cluster's histogram, a bin a thread, and the first bin at which the running count (or mass) reaches `goal`: into
-    // s.found_*: the bin, what lies before it, its size.  total_mass: of all bins.  goal 0 looks for the mass's total only.
-    __device__ void find(bool by_mass, u64 before_count, u64 before_mass, u64 goal) {
+    // The count or the mass that a cut by mass has to reach, out of `total`.
+    __device__ static u64 share_of(double p, u64 total) {
+        const double want = ceil(fmax(p, 0.0) * (double)total);
+        return want < 1.0 ? 1ull : min((u64)want, total);
+    }
+    // The cluster's histogram, a bin a thread, and the first bin at which the running count (or mass) reaches the goal: into
+    // s.found_*: the bin (kBins: none), what lies before it, its count.  goal 0: the share p of the mass without `out` of it.
+    __device__ u64 find(bool by_mass, u64 before, u64 goal, double p, u64 out) {
         meet(a.ranks);
         clear(hist_turn ^ 1);                            // every CTA is past its reads of that one
-        uint32_t count = 0;
-        u64 mass = 0;
-        const uint32_t at = shared_addr(&s.hist[hist_turn][threadIdx.x]);
-        for (int r = 0; r < a.ranks; ++r) {
-            const uint4 h = a.ranks > 1 ? ld_rank(of_rank(at, r)) : s.hist[hist_turn][threadIdx.x];
-            count += h.x;
-            mass += (u64)h.y + ((u64)h.z << 16) + ((u64)h.w << 32);
-        }
-        hist_turn ^= 1;
-        uint32_t c = count;
-        u64 m = mass;
+        u64 own = 0;
+        const uint32_t at_count = shared_addr(&s.count[hist_turn][threadIdx.x]), at_mass = shared_addr(&s.mass[hist_turn][threadIdx.x]);
+        u64 h[kMaxRanks];                                // all of them asked for before the first is used
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const uint32_t oc = __shfl_up_sync(0xffffffffu, c, d);
-            const u64 om = __shfl_up_sync(0xffffffffu, m, d);
-            if (lane >= d) { c += oc; m += om; }
+        for (int r = 0; r < kMaxRanks; ++r) {
+            h[r] = 0;
+            if (r < a.ranks) {
+                if (by_mass) h[r] = ld_rank64(of_rank(at_mass, r));
+                else h[r] = ld_rank32(of_rank(at_count, r));
+            }
         }
-        if (lane == 31) { s.warp_count[warp] = c; s.warp_mass[warp] = m; }
+#pragma unroll
+        for (int r = 0; r < kMaxRanks; ++r) own += h[r];
+        const int turn = hist_turn;
+        hist_turn ^= 1;
+        const u64 up = add_up(own);
+        if (lane == 31) s.warp_mass[warp] = up;
         if (threadIdx.x == 0) s.found_bin = kBins;
         __syncthreads();
-        u64 pc = before_count, pm = before_mass, all = before_mass;
-        for (int w = 0; w < kSampleWarps; ++w) {
-            if (w < warp) { pc += s.warp_count[w]; pm += s.warp_mass[w]; }
-            all += s.warp_mass[w];
+        u64 ahead = add_up(s.warp_mass[lane]);           // the warps' sums, added up by every warp
+        if (goal == 0) goal = share_of(p, before + __shfl_sync(0xffffffffu, ahead, 31) - out);
+        ahead = __shfl_sync(0xffffffffu, ahead, warp > 0 ? warp - 1 : 0);
+        const u64 hi = before + (warp > 0 ? ahead : 0) + up, lo = hi - own;
+        if (lo < goal && goal <= hi) {
+            uint32_t n = (uint32_t)own;
+            if (by_mass) {
+                n = 0;
+#pragma unroll 1
+                for (int r = 0; r < a.ranks; ++r) n += ld_rank32(of_rank(shared_addr(&s.count[turn][threadIdx.x]), r));
+            }
+            s.found_bin = threadIdx.x;
+            s.found_before = lo;
+            s.found_size = n;
         }
-        const u64 hi_c = pc + c, hi_m = pm + m, lo_c = hi_c - count, lo_m = hi_m - mass;
-        const bool here = by_mass ? lo_m < goal && goal <= hi_m : lo_c < goal && goal <= hi_c;
-        if (here) { s.found_bin = threadIdx.x; s.found_count = (uint32_t)lo_c; s.found_mass = lo_m; s.found_size = count; }
-        if (threadIdx.x == 0) s.total_mass = all;
         __syncthreads();
-    }
-
-    // From the linear bin s.found_bin down to one value.  `from`: only keys of at least that.
-    __device__ Cut narrow(bool by_mass, u64 goal, uint32_t from) {
-        const uint32_t bin = s.found_bin;
-        u64 count = s.found_count, mass = s.found_mass;
-        uint32_t size = s.found_size;
-        // keys that the bin can hold: its edges, moved out by more than rounding moved them
-        const float width = 1.0f / bin_scale;
-        const float x_hi = largest - (float)bin * width * 0.9999f, x_lo = largest - ((float)bin + 1.0f) * width * 1.0001f;
-        uint32_t hi = Row<T>::key(bin == 0 ? largest : fminf(x_hi + fabsf(largest) * 1e-6f, largest));
-        uint32_t lo = isinf(largest) ? hi : Row<T>::key(x_lo - fabsf(largest) * 1e-6f);
-        if (lo < from) lo = from;
-        __syncthreads();                                 // found_* has been read
-        for (int level = 0; level < 4; ++level) {        // 32 bits, 10 a level
-            const uint32_t span = hi - lo;
-            const int shift = span < (uint32_t)kBins ? 0 : 22 - __clz(span);
-            const int which = hist_turn;
-            each([&](float x, int) {
-                if (linear(x) != bin) return;
-                const uint32_t k = Row<T>::key(x);
-                if (k >= lo && k <= hi) put(which, (hi - k) >> shift, by_mass, x);
-            });
-            find(by_mass, count, mass, goal);
-            const uint32_t b = s.found_bin;
-            count = s.found_count; mass = s.found_mass; size = s.found_size;
-            __syncthreads();
-            hi -= b << shift;
-            if (shift == 0) break;
-            const uint32_t width_keys = 1u << shift;
-            if (hi - lo >= width_keys) lo = hi - width_keys + 1;
-        }
-        Cut cut;
-        cut.key = hi;
-        cut.equal = size;
-        cut.ties = (uint32_t)(goal - count);
-        if (by_mass) {                                   // equal weights: as many as are needed
-            const u64 w = fixed(value_of(hi));
-            cut.ties = (uint32_t)((goal - mass + w - 1) / w);
-        }
-        return cut;
+        return goal;
     }
     __device__ static float value_of(uint32_t key) {
         if constexpr (sizeof(T) == 4) {
@@ -270,48 +305,122 @@ struct Sampler {
             return Elem<T>::load(reinterpret_cast<const T*>(&b));
         }
     }
+    __device__ u64 block_sum(u64 v) {
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+        if (lane == 0) s.warp_mass[warp] = v;
+        __syncthreads();
+        u64 all = s.warp_mass[lane];
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) all += __shfl_xor_sync(0xffffffffu, all, d);
+        __syncthreads();
+        return all;
+    }
+    __device__ u64 target_of(double u, u64 total) const {
+        const double want = u > 0.0 ? u * (double)total : 0.0;
+        return want < (double)total ? min((u64)want, total - 1) : total - 1;
+    }
+    __device__ void answer(int64_t r, int index, float x, bool greedy, u64 total) const {
+        a.token[r] = index;
+        if (a.logprob) a.logprob[r] = greedy ? 0.0f : (float)((x == largest ? 0.0 : ((double)x - top) * inv_t) - log_of(total));
+    }
+
+    // At most kFew candidates, the elements of the linear bins up to `bin`: rank 0 takes them all, four threads to each, and
+    // adds up what goes before it, by value and then, of the kept ones, by index.
+    __device__ void choose_from_few(int64_t r, uint32_t bin, uint32_t k, double p, u64 lowest, double u) {
+        const uint32_t count_at = of_rank(shared_addr(&s.few_count), 0), few_at = of_rank(shared_addr(s.few), 0);
+#pragma unroll 1
+        for (int c = c0 + lane; c < c1; c += 32) {
+            float x[4];
+            get(c, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (x[j] < floor_x || linear(x[j]) > bin) continue;
+                const uint32_t at = add_rank32(count_at, 1), index = (uint32_t)(c * 4 + j - skew);
+                if (at < kFew) st_rank64(few_at + at * 8, (u64)Row<T>::key(x[j]) << 32 | (uint32_t)~index);
+            }
+        }
+        meet(a.ranks);
+        if (rank != 0) return;
+        const uint32_t n = min(s.few_count, kFew), i = threadIdx.x / 4, part = threadIdx.x % 4;
+        if (threadIdx.x < n) s.few_weight[threadIdx.x] = weight(value_of((uint32_t)(s.few[threadIdx.x] >> 32)));
+        __syncthreads();
+        const u64 order = i < n ? s.few[i] : 0, w = i < n ? s.few_weight[i] : 0;
+        const float x = value_of((uint32_t)(order >> 32));
+        auto four = [](u64 v) {
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            return v + __shfl_xor_sync(0xffffffffu, v, 2);
+        };
+        u64 mass = 0;
+        uint32_t ahead = 0;
+#pragma unroll 2
+        for (uint32_t j = part; j < n; j += 4) {
+            const bool before = s.few[j] > order;
+            mass += before ? s.few_weight[j] : 0;
+            ahead += before;
+        }
+        mass = four(mass);
+        ahead = (uint32_t)four(ahead);
+        bool kept = i < n && ahead < k;
+        const u64 of_k = block_sum(kept && part == 0 ? w : 0);
+        kept = kept && (p >= 1.0 || mass < share_of(p, of_k)) && w >= lowest;
+        if (part == 0 && i < n) s.few_weight[i] = kept ? w : 0;
+        const u64 total = block_sum(kept && part == 0 ? w : 0), goal = target_of(u, total);
+        u64 at = 0;
+#pragma unroll 2
+        for (uint32_t j = part; j < n; j += 4) at += (uint32_t)s.few[j] > (uint32_t)order ? s.few_weight[j] : 0;      // a lower index
+        at = four(at);
+        if (part == 0 && kept && goal >= at && goal < at + w) answer(r, (int)~(uint32_t)order, x, false, total);
+    }
 
     __device__ void run(int64_t r) {
         const int ranks = a.ranks;
+        const double t = a.temperature.of(r), p = a.top_p.of(r), u = (double)__ldg(a.uniform + r);
+        const int k = a.top_k.of(r);
+        const bool greedy = !(t > 0.0);
+        const u64 lowest = greedy ? 0 : (u64)__double2ll_rn(fmin(fmax(a.min_p.of(r), 0.0), 1.0) * kOne);
         // the row's granules, the cluster's share, the warps' shares: contiguous, so that indices rise with rank, warp, lane
-        const int per_rank = (granules + ranks - 1) / ranks;
-        base = min(rank * per_rank, granules);
-        const int end = min(base + per_rank, granules), per_warp = (end - base + kSampleWarps - 1) / kSampleWarps;
-        g0 = min(base + warp * per_warp, end);
-        g1 = min(g0 + per_warp, end);
-        turn = 0;
+        const int granules = (a.vocab + skew + kPer - 1) / kPer, per_rank = (granules + ranks - 1) / ranks;
+        first = min(rank * per_rank, granules);
+        const int end = min(first + per_rank, granules), per_warp = (end - first + kSampleWarps - 1) / kSampleWarps;
+        const int g0 = min(first + warp * per_warp, end), g1 = min(g0 + per_warp, end);
+        c0 = g0 * (kPer / 4);
+        c1 = g1 * (kPer / 4);
         hist_turn = 0;
         clear(0);
         clear(1);
+        if (threadIdx.x < kSteps) s.octave[threadIdx.x] = octave_step(threadIdx.x);
+        if (threadIdx.x == 0) s.few_count = 0;
 
-        float top = kNegInf;
-        for (int g = g0 + lane; g < g1; g += 32) {
-            float v[kPer];
-            fetch(g, v);
-            if constexpr (kResident) {
-                T e[kPer];
+        float most = kNegInf;
+        constexpr int kAhead = 4;                        // granules of a lane on their way at once
+#pragma unroll 1
+        for (int g = g0 + lane; g < g1; g += 32 * kAhead) {
+            uint4 v[kAhead];
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) e[j] = Elem<T>::round(v[j]);
-                held[g - base] = *reinterpret_cast<const uint4*>(e);
+            for (int i = 0; i < kAhead; ++i) v[i] = fetch(min(g + 32 * i, g1 - 1));
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if constexpr (kResident) held[min(g + 32 * i, g1 - 1) - first] = v[i];
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) most = fmaxf(most, Elem<T>::load(reinterpret_cast<const T*>(&v[i]) + j));
             }
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) top = fmaxf(top, v[j]);
         }
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        if (lane == 0) s.warp_max[warp] = top;
+        for (int d = 16; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        if (lane == 0) s.warp_max[warp] = most;
         __syncthreads();
         if (warp == 0) {
-            top = s.warp_max[lane];
+            most = s.warp_max[lane];
 #pragma unroll
-            for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            if (lane < ranks) st_rank32(of_rank(shared_addr(&s.slots[0].largest[rank]), lane), __float_as_uint(top));
+            for (int d = 16; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            if (lane < ranks) st_rank32(of_rank(shared_addr(&s.slots[0].largest[rank]), lane), __float_as_uint(most));
         }
         meet(ranks);
-        turn = 1;
         largest = kNegInf;
+#pragma unroll 1
         for (int q = 0; q < ranks; ++q) largest = fmaxf(largest, s.slots[0].largest[q]);
-
+        top = (double)fminf(largest, FLT_MAX);
         if (largest == kNegInf) {                        // nothing to choose from
             if (rank == 0 && threadIdx.x == 0) {
                 a.token[r] = -1;
@@ -319,157 +428,186 @@ struct Sampler {
             }
             return;
         }
-        const double t = a.temperature.of(r);
-        const bool greedy = !(t > 0.0);
         inv_t = greedy ? 1.0 : 1.0 / t;
-        bin_scale = greedy ? 1.0f : (float)fmin((double)kBins / (kSpan * t), 1e38);
-        const int k = a.top_k.of(r);
-        const double p = a.top_p.of(r), lowest = greedy ? 0.0 : fmin(a.min_p.of(r), 1.0);
-        Cut cut{0, 0, 0};                                // key 0: everything
-        if (greedy) {
-            cut = Cut{Row<T>::key(largest), 1, 0xffffffffu};
-        } else {
-            if (k > 0 && k < a.vocab) {
-                each([&](float x, int) {
-                    const uint32_t bin = linear(x);
-                    if (bin < (uint32_t)kBins) put(hist_turn, bin, false, x);
-                });
-                find(false, 0, 0, (u64)k);
-                if (s.found_bin < (uint32_t)kBins) cut = narrow(false, (u64)k, 0);      // else fewer than k have a weight
+        steps_t = inv_t * (kSteps * 1.4426950408889634074);
+        bin_scale = (float)fmin((double)kBins / kSpan * inv_t, 1e38);
+        floor_x = greedy || isinf(largest) ? largest : fmaxf((float)(top - kSpan * t), -FLT_MAX);
+
+        // The cut, first by count, then by mass within what that kept; each by linear bins, then by keys in the bin found.
+        Cut cut{floor_x, 0, 0};                          // everything
+        if (greedy) cut = Cut{largest, 1, 0xffffffffu};
+#pragma unroll 1
+        for (int stage = k > 0 && k < a.vocab ? 0 : 1; stage < (greedy ? 0 : p < 1.0 ? 2 : 1); ++stage) {
+            const bool by_mass = stage == 1;
+            // the mass of the equal values that the cut by count leaves out
+            const u64 out = by_mass && cut.equal > cut.ties ? (u64)(cut.equal - cut.ties) * weight(cut.value) : 0;
+            u64 goal = by_mass ? 0 : (u64)k, before = 0;
+            uint32_t bin = 0, lo = 0, hi = 0;
+#pragma unroll 1
+            for (int level = 0; level < 5; ++level) {    // 32 bits of a key, 10 a level
+                const uint32_t span = hi - lo;
+                const int shift = span < (uint32_t)kBins ? 0 : 22 - __clz(span);
+#pragma unroll 1
+                for (int c = c0 + lane; c < c1; c += 32) {
+                    float x[4];
+                    get(c, x);
+                    uint32_t at[4];
+                    bool hit[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        at[j] = linear(x[j]);
+                        hit[j] = x[j] >= cut.value && (level == 0 || at[j] == bin);
+                    }
+                    if (!(hit[0] || hit[1] || hit[2] || hit[3])) continue;
+                    if (level > 0) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t key = Row<T>::key(x[j]);
+                            hit[j] = hit[j] && key >= lo && key <= hi;
+                            at[j] = (hi - key) >> shift;
+                        }
+                    }
+                    u64 w[4] = {};
+                    if (by_mass) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) w[j] = weight(fmaxf(x[j], floor_x));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (hit[j]) put(at[j], !by_mass || level > 0, w[j]);
+                }
+                goal = find(by_mass, before, goal, p, out);
+                const uint32_t b = s.found_bin;
+                before = s.found_before;
+                const uint32_t size = s.found_size;
+                if (b == (uint32_t)kBins) break;         // fewer than k have a weight: all of them stay
+                if (level == 0) {
+                    if (!by_mass && before + size <= kFew) return choose_from_few(r, b, (uint32_t)k, p, lowest, u);
+                    // keys that the bin can hold: its edges, moved out by more than rounding moved them
+                    bin = b;
+                    const float width = 1.0f / bin_scale;
+                    const float x_hi = largest - (float)bin * width * 0.9999f, x_lo = largest - ((float)bin + 1.0f) * width * 1.0001f;
+                    hi = Row<T>::key(bin == 0 ? largest : fminf(x_hi + fabsf(largest) * 1e-6f, largest));
+                    lo = isinf(largest) ? hi : Row<T>::key(cut.value);
+                    if (bin < (uint32_t)kBins - 1) lo = max(lo, Row<T>::key(x_lo - fabsf(largest) * 1e-6f));
+                } else {
+                    hi -= b << shift;
+                    if (shift == 0) {
+                        const u64 w = by_mass ? weight(value_of(hi)) : 1;
+                        cut = Cut{value_of(hi), (uint32_t)((goal - before + w - 1) / w), size};      // equal weights: as many as are needed
+                        break;
+                    }
+                    if (hi - lo >= 1u << shift) lo = hi - (1u << shift) + 1;
+                }
+                __syncthreads();                         // found_* has been read
             }
-            if (p < 1.0) {
-                each([&](float x, int) {
-                    const uint32_t bin = linear(x);
-                    if (bin < (uint32_t)kBins && Row<T>::key(x) >= cut.key) put(hist_turn, bin, true, x);
-                });
-                // two looks at the same histogram: the sum, then the bin
-                find(true, 0, 0, 0);
-                u64 total = s.total_mass;
-                if (cut.key) total -= (u64)(cut.equal - cut.ties) * fixed(value_of(cut.key));
-                const double want = ceil(fmax(p, 0.0) * (double)total);
-                u64 goal = want < 1.0 ? 1 : (u64)want;
-                if (goal > total) goal = total;
-                hist_turn ^= 1;                          // the same one again
-                find(true, 0, 0, goal);
-                cut = narrow(true, goal, cut.key);
-            }
+            __syncthreads();
         }
 
         // equal values before this warp's
         uint32_t ties_before = 0, ties_here = 0;
         const bool some = cut.ties < cut.equal;          // not all of them are kept
         if (some) {
-            each([&](float x, int) { ties_here += x > kNegInf && Row<T>::key(x) == cut.key; });
+#pragma unroll 1
+            for (int c = c0 + lane; c < c1; c += 32) {
+                float x[4];
+                get(c, x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ties_here += x[j] == cut.value;
+            }
             ties_here = __reduce_add_sync(0xffffffffu, ties_here);
-            __syncthreads();
             if (lane == 0) s.warp_count[warp] = ties_here;
             __syncthreads();
+            const uint32_t up = (uint32_t)add_up(s.warp_count[lane]);
             if (warp == 0) {
-                const uint32_t sum = __reduce_add_sync(0xffffffffu, s.warp_count[lane]);
-                if (lane < ranks) st_rank32(of_rank(shared_addr(&s.slots[turn].count[rank]), lane), sum);
+                const uint32_t all = __shfl_sync(0xffffffffu, up, 31);
+                if (lane < ranks) st_rank32(of_rank(shared_addr(&s.slots[1].count[rank]), lane), all);
             }
+            ties_before = __shfl_sync(0xffffffffu, up, warp > 0 ? warp - 1 : 0);
+            if (warp == 0) ties_before = 0;
             meet(ranks);
-            for (int q = 0; q < rank; ++q) ties_before += s.slots[turn].count[q];
-            for (int w = 0; w < warp; ++w) ties_before += s.warp_count[w];
-            turn ^= 1;
+#pragma unroll 1
+            for (int q = 0; q < rank; ++q) ties_before += s.slots[1].count[q];
         }
-        // the weight of an element if it is kept; ties of this warp that come before it
-        auto kept = [&](float x, uint32_t tie) -> u64 {
-            if (x == kNegInf) return 0;
-            const uint32_t key = Row<T>::key(x);
-            if (key < cut.key || (some && key == cut.key && ties_before + tie >= cut.ties)) return 0;
-            const double w = weight(x);
-            return w >= lowest ? (u64)__double2ll_rn(w * kOne) : 0;
-        };
-        // Elements of a step (32 granules) before this lane's that are equal to the cut's value.
-        auto tie_rank = [&](const float (&v)[kPer], bool in, uint32_t& running) -> uint32_t {
-            uint32_t n = 0;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) n += in && v[j] > kNegInf && Row<T>::key(v[j]) == cut.key;
-            uint32_t up = n;
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const uint32_t o = __shfl_up_sync(0xffffffffu, up, d);
-                if (lane >= d) up += o;
-            }
-            const uint32_t mine = running + up - n;
-            running += __shfl_sync(0xffffffffu, up, 31);
-            return mine;
-        };
         const bool cut_here = some && ties_before < cut.ties && ties_before + ties_here > cut.ties;
-        u64 sum = 0;
-        uint32_t running = 0;
-        for (int g = g0; g < g1; g += 32) {
-            const bool in = g + lane < g1;
-            float v[kPer];
-            if (in) get(g + lane, base, v);
-            uint32_t tie = cut_here ? tie_rank(v, in, running) : 0;
-            if (in) {
+        // Twice over the warp's elements: every warp adds its kept weights up, then the one whose sum the target falls in looks
+        // for the token.  One copy of the code for both.
+        u64 before = 0, goal = 0, total = 0;
+#pragma unroll 1
+        for (int look = 0; look < 2; ++look) {
+            u64 sum = 0;
+            uint32_t running = 0;
+#pragma unroll 1
+            for (int c = c0; c < c1; c += 32) {
+                const bool in = c + lane < c1;
+                float x[4];
+                get(min(c + lane, c1 - 1), x);
+                bool hit[4], equal[4];
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) {
-                    sum += kept(v[j], tie);
-                    if (cut_here) tie += v[j] > kNegInf && Row<T>::key(v[j]) == cut.key;
+                for (int j = 0; j < 4; ++j) {
+                    hit[j] = in && x[j] >= cut.value;
+                    equal[j] = hit[j] && x[j] == cut.value;
                 }
-            }
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        __syncthreads();
-        if (lane == 0) s.warp_mass[warp] = sum;
-        __syncthreads();
-        if (warp == 0) {
-            u64 all = s.warp_mass[lane];
-#pragma unroll
-            for (int d = 16; d > 0; d /= 2) all += __shfl_xor_sync(0xffffffffu, all, d);
-            if (lane < ranks) st_rank64(of_rank(shared_addr(&s.slots[turn].mass[rank]), lane), all);
-        }
-        meet(ranks);
-        u64 total = 0, before = 0;
-        for (int q = 0; q < ranks; ++q) {
-            if (q < rank) before += s.slots[turn].mass[q];
-            total += s.slots[turn].mass[q];
-        }
-        for (int w = 0; w < warp; ++w) before += s.warp_mass[w];
-        const double u = (double)__ldg(a.uniform + r);
-        const double want = u > 0.0 ? u * (double)total : 0.0;
-        const u64 goal = want < (double)total ? min((u64)want, total - 1) : total - 1;
-        if (goal < before || goal >= before + sum) return;          // another warp's
-        // this warp holds the token: lanes' sums of a step, then the elements of the lane
-        running = 0;
-        for (int g = g0; g < g1; g += 32) {
-            const bool in = g + lane < g1;
-            float v[kPer];
-            if (in) get(g + lane, base, v);
-            uint32_t tie = cut_here ? tie_rank(v, in, running) : 0;
-            u64 w[kPer], mine = 0;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                w[j] = in ? kept(v[j], tie) : 0;
-                if (cut_here) tie += in && v[j] > kNegInf && Row<T>::key(v[j]) == cut.key;
-                mine += w[j];
-            }
-            u64 up = mine;
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const u64 o = __shfl_up_sync(0xffffffffu, up, d);
-                if (lane >= d) up += o;
-            }
-            u64 at = before + up - mine;
-            before += __shfl_sync(0xffffffffu, up, 31);
-            if (goal >= at && goal < at + mine) {
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) {
-                    if (goal >= at && goal < at + w[j]) {
-                        a.token[r] = (long long)(g + lane) * kPer + j - skew;
-                        if (a.logprob)
-                            a.logprob[r] = greedy ? 0.0f
-                                                  : (float)((v[j] == largest ? 0.0 : ((double)v[j] - (double)largest) * inv_t) -
-                                                            log((double)total / kOne));
+                if (!__any_sync(0xffffffffu, hit[0] || hit[1] || hit[2] || hit[3])) continue;
+                if (some) {
+                    uint32_t tie = ties_before;
+                    if (cut_here) {                      // equal values of this warp before this lane's
+                        const uint32_t n = equal[0] + equal[1] + equal[2] + equal[3], up = (uint32_t)add_up(n);
+                        tie += running + up - n;
+                        running += __shfl_sync(0xffffffffu, up, 31);
                     }
-                    at += w[j];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        hit[j] = hit[j] && !(equal[j] && tie >= cut.ties);
+                        tie += equal[j];
+                    }
                 }
+                u64 w[4], mine = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w[j] = weight(fmaxf(x[j], floor_x));
+                    if (!hit[j] || w[j] < lowest) w[j] = 0;
+                    mine += w[j];
+                }
+                if (look == 0) {
+                    sum += mine;
+                    continue;
+                }
+                const u64 up = add_up(mine);
+                u64 at = before + up - mine;
+                before += __shfl_sync(0xffffffffu, up, 31);
+                if (goal >= at && goal < at + mine) {
+                    int index = 0;
+                    float value = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (goal >= at && goal < at + w[j]) { index = j; value = x[j]; }
+                        at += w[j];
+                    }
+                    answer(r, (c + lane) * 4 + index - skew, value, greedy, total);
+                }
+                if (goal < before) break;
             }
-            if (goal < before) break;
+            if (look == 1) break;
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            if (lane == 0) s.warp_mass[warp] = sum;
+            __syncthreads();
+            const u64 up = add_up(s.warp_mass[lane]);
+            if (warp == 0) {
+                const u64 all = __shfl_sync(0xffffffffu, up, 31);
+                if (lane < ranks) st_rank64(of_rank(shared_addr(&s.slots[0].mass[rank]), lane), all);
+            }
+            before = __shfl_sync(0xffffffffu, up, warp > 0 ? warp - 1 : 0);
+            if (warp == 0) before = 0;
+            meet(ranks);
+#pragma unroll 1
+            for (int q = 0; q < ranks; ++q) {
+                if (q < rank) before += s.slots[0].mass[q];
+                total += s.slots[0].mass[q];
+            }
+            goal = target_of(u, total);
+            if (goal < before || goal >= before + sum) break;          // another warp's
         }
     }
 };
@@ -484,7 +622,6 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleA
     one.held = reinterpret_cast<uint4*>(sample_smem);
     one.row = row;
     one.skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-    one.granules = (a.vocab + one.skew + one.kPer - 1) / one.kPer;
     one.warp = threadIdx.x >> 5;
     one.lane = threadIdx.x & 31;
     one.rank = (int)(blockIdx.x % a.ranks);
