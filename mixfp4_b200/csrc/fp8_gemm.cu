@@ -11,7 +11,7 @@
 //   swapped  (up to 64 rows of x) the lanes are weight rows, the columns 16, 32 or 64 rows of x, so that no tensor time
 //            and no bandwidth is spent on rows that are not there; a block's scales come as a row of shared memory.
 //
-//   warps 0 .. E-1   epilogue (E = 4, or 8 with 128 columns and more)
+//   warps 0 .. E-1   epilogue (E = 4, 8 with 128 columns, 16 with 256)
 //   warp E           producer: per block of 128 K a box of both operands (128-byte swizzle) and the scales of x
 //   warp E + 1       tensor memory, MMA issue
 //
@@ -38,18 +38,18 @@ struct Fp8Args {
     int64_t ldsx, ldy;
     int m, n, blocks;
     int x_tiles, items, cluster, stages, out_dtype;
-    bool y_vec;                          // rows of y are 16-byte aligned
+    bool y_vec;                          // rows of y are 32-byte aligned
     int* status;
 };
 
 template <int kCols, bool kSwap>
 struct Fp8Cfg {
-    static constexpr int kEpi = kCols > 64 ? 8 : 4;                     // epilogue warps
+    static constexpr int kEpi = kCols > 64 ? 8 : 4;                     // epilogue warps: 64 columns a thread at most
     static constexpr int kPer = kCols * 4 / kEpi;                       // columns of a thread
     static constexpr int kThreads = (kEpi + 2) * 32;
     static constexpr uint32_t kABytes = 128 * 128, kBBytes = kCols * 128, kStage = kABytes + kBBytes;
-    static constexpr int kScales = kSwap ? kCols : 128;                 // scales of x in a block
-    static constexpr int kBufs = kCols > 128 ? 2 : 4;
+    static constexpr int kScales = kSwap ? kCols : 0;                   // scales of x in a stage
+    static constexpr int kBufs = 4;
     static constexpr uint32_t kBufCols = kCols < 32 ? 32 : kCols, kTmemCols = kBufs * kBufCols;
     // D fp32, A and B E4M3, both K-major
     static constexpr uint32_t kInstrDesc = (1u << 4) | ((uint32_t)(kCols >> 3) << 17) | ((128u >> 4) << 24);
@@ -83,30 +83,33 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-// kN columns of this warp's 32 lanes, without the wait.
-template <int kN>
-__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&r)[kN]);
-template <>
-__device__ __forceinline__ void tmem_load<16>(uint32_t taddr, float (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
-        : "r"(taddr) : "memory");
+// 16 or 32 columns of this warp's 32 lanes, without the wait.
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
 }
-// The values may be used after this; they pass through it so that no use moves above it.
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// A loaded column passes through this after the wait, so that no use of it moves above.
 template <int kN>
-__device__ __forceinline__ void tmem_wait(float (&r)[kN]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+__device__ __forceinline__ void tmem_landed(uint32_t (&r)[kN]) {
 #pragma unroll
-    for (int i = 0; i < kN; ++i) asm volatile("" : "+f"(r[i]));
+    for (int i = 0; i < kN; ++i) asm volatile("" : "+r"(r[i]));
 }
+template <int kRegs>
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+template <int kRegs>
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 
-__device__ __forceinline__ float lds_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-    return v;
-}
 __device__ __forceinline__ float4 lds_f32x4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
@@ -156,25 +159,35 @@ __device__ __forceinline__ void store_one(const Fp8Args& a, int64_t row, int64_t
     else if (a.out_dtype == MIXFP4_BF16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
     else static_cast<__half*>(a.y)[at] = __float2half_rn(v);
 }
-// kN consecutive columns of a row, 16 bytes at a time where the whole run is inside and aligned.
+// 32 aligned bytes, a whole sector of the L2.
+__device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+// kN consecutive columns of a row, a sector at a time where the whole run is inside and aligned.
 template <int kN>
 __device__ __forceinline__ void store_run(const Fp8Args& a, int64_t row, int64_t col, const float (&v)[kN]) {
-    static_assert(kN % 8 == 0, "a run is stored in 16-byte pieces");
+    static_assert(kN % 16 == 0, "a run is stored in sectors");
     if (!a.y_vec || col + kN > a.n) {
 #pragma unroll
         for (int j = 0; j < kN; ++j)
             if (col + j < a.n) store_one(a, row, col + j, v[j]);
     } else if (a.out_dtype == MIXFP4_F32) {
-        float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.y) + row * a.ldy + col);
-#pragma unroll
-        for (int j = 0; j < kN; j += 4) p[j / 4] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-    } else {
-        uint4* p = reinterpret_cast<uint4*>(static_cast<__half*>(a.y) + row * a.ldy + col);
+        float* p = static_cast<float*>(a.y) + row * a.ldy + col;
 #pragma unroll
         for (int j = 0; j < kN; j += 8) {
-            uint32_t w[4];
+            uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[j + i]);
+            st_sector(p + j, w);
+        }
+    } else {
+        __half* p = static_cast<__half*>(a.y) + row * a.ldy + col;
+#pragma unroll
+        for (int j = 0; j < kN; j += 16) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
                 const float lo = v[j + 2 * i], hi = v[j + 2 * i + 1];
                 if (a.out_dtype == MIXFP4_BF16) {
                     const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
@@ -184,8 +197,50 @@ __device__ __forceinline__ void store_run(const Fp8Args& a, int64_t row, int64_t
                     w[i] = *reinterpret_cast<const uint32_t*>(&h);
                 }
             }
-            p[j / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+            st_sector(p + j, w);
         }
+    }
+}
+
+// acc += columns src .. of this warp's lanes * f, the next 32 columns on their way while 32 are added; given_back() once the
+// last have landed.  (One multiplication at a time: the packed form of two needs its operands in aligned pairs, and the moves
+// that bring the loaded columns there cost more than it saves.)
+template <int kPer, typename Done>
+__device__ __forceinline__ void add_scaled(uint32_t src, float f, float (&acc)[kPer], Done&& given_back) {
+    uint32_t v[2][32];
+    tmem_load(src, v[0]);
+#pragma unroll
+    for (int c = 0; c < kPer; c += 32) {
+        tmem_wait();
+        tmem_landed(v[(c / 32) & 1]);
+        if (c + 32 < kPer) tmem_load(src + c + 32, v[(c / 32 + 1) & 1]);
+        else given_back();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(__uint_as_float(v[(c / 32) & 1][j]), f, acc[c + j]);
+    }
+}
+// The same with a scale for every column, at sc in shared memory, times sw.
+template <int kPer, typename Done>
+__device__ __forceinline__ void add_scaled_by_column(uint32_t src, uint32_t sc, float sw, float (&acc)[kPer], Done&& given_back) {
+    constexpr int kLoad = kPer < 32 ? kPer : 32;
+    uint32_t v[kPer / kLoad][kLoad];
+    float4 sj[kPer / 4];
+#pragma unroll
+    for (int c = 0; c < kPer; c += kLoad) tmem_load(src + c, v[c / kLoad]);
+#pragma unroll
+    for (int q = 0; q < kPer / 4; ++q) sj[q] = lds_f32x4(sc + q * 16);
+    tmem_wait();
+#pragma unroll
+    for (int c = 0; c < kPer; c += kLoad) tmem_landed(v[c / kLoad]);
+#pragma unroll
+    for (int q = 0; q < kPer / 4; ++q)                              // the scales have been read before the stage is given back
+        asm volatile("" : "+f"(sj[q].x), "+f"(sj[q].y), "+f"(sj[q].z), "+f"(sj[q].w));
+    given_back();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const float4 four = sj[j / 4];
+        const float f = (j % 4 == 0 ? four.x : j % 4 == 1 ? four.y : j % 4 == 2 ? four.z : four.w) * sw;
+        acc[j] = fmaf(__uint_as_float(v[j / kLoad][j % kLoad]), f, acc[j]);
     }
 }
 
@@ -208,7 +263,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     const WaitCtx ctx{abort_flag, a.status};
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < a.stages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1 + C::kEpi); }
+        for (int s = 0; s < a.stages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), kSwap ? 1 + C::kEpi : 1); }
         for (int b = 0; b < C::kBufs; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), C::kEpi); }
         mbar_init(sums_in, (uint32_t)a.cluster * C::kEpi);              // every warp of every CTA of the cluster has sent
         mbar_init(sums_out, (uint32_t)a.cluster * C::kEpi);             // ... and has added its share of what was sent
@@ -227,8 +282,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     const int k0 = a.blocks * rank / a.cluster, k1 = a.blocks * (rank + 1) / a.cluster;
     const int step = (int)gridDim.x / a.cluster, first = (int)blockIdx.x / a.cluster;
 
-    if (warp == C::kEpi) {
-        if (lane == 0) {
+    if (warp >= C::kEpi) {
+        if (warp == C::kEpi && lane == 0) {
             // Weights never depend on the kernel before (the quantizer of x): the first round of stages asks for them ahead of the wait.
             int s = 0, ahead = 0;
             uint32_t ph = 0;
@@ -252,13 +307,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                         weights(item, kb, s);
                     }
                     tma_load_2d(base + s * C::kStage + (kSwap ? C::kABytes : 0u), &map_x, full(s), kb * 128, x0);
-                    bulk_load(base + L.scales + s * (C::kScales * 4), a.sx + (int64_t)kb * a.ldsx + x0, C::kScales * 4, full(s));
+                    if constexpr (kSwap)
+                        bulk_load(base + L.scales + s * (C::kScales * 4), a.sx + (int64_t)kb * a.ldsx + x0, C::kScales * 4, full(s));
                     if (++s == a.stages) { s = 0; ph ^= 1; }
                 }
             }
         }
-    } else if (warp == C::kEpi + 1) {
-        if (lane == 0) {
+        if (warp == C::kEpi + 1 && lane == 0) {
             int s = 0, b = 0;
             uint32_t ph = 0, bph = 0;
             bool ok = true;
@@ -279,6 +334,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             }
         }
     } else {
+        if constexpr (!kSwap) asm volatile("griddepcontrol.wait;" ::: "memory");     // the scales are the kernel before's
         const int quad = warp & 3, half = warp >> 2;                    // lanes 32 quad .., columns half * kPer ..
         const int tl = quad * 32 + lane;
         int s = 0, b = 0;
@@ -291,35 +347,43 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             float acc[C::kPer];
 #pragma unroll
             for (int j = 0; j < C::kPer; ++j) acc[j] = 0.0f;
-            float sw_next = k0 < k1 ? __ldg(sw + k0) : 0.0f;
-            for (int kb = k0; kb < k1; ++kb) {
-                const float sw_now = sw_next;
-                if (kb + 1 < k1) sw_next = __ldg(sw + kb + 1);
-                ok = __all_sync(0xffffffffu, mbar_wait(acc_full(b), bph, ctx, 24) && mbar_wait(full(s), ph, ctx, 25));
+            // Scales on their way kFar blocks ahead, in registers that take turns (moving one on would wait for it).  (They are not a stage's: a stage that stays until its scales have
+            // been read keeps the operands behind it waiting.)
+            constexpr int kFar = 4;
+            const float *sx = a.sx + min(x0 + tl, a.m - 1) + k0 * a.ldsx, *sw_at = sw + k0;
+            float sx_far[kFar], sw_far[kFar];
+            auto fetch_scales = [&](int i, bool more) {
+                if (more) {
+                    sw_far[i] = __ldg(sw_at);
+                    if constexpr (!kSwap) sx_far[i] = __ldcg(sx);
+                }
+                ++sw_at;
+                if constexpr (!kSwap) sx += a.ldsx;
+            };
+#pragma unroll
+            for (int i = 0; i < kFar; ++i) fetch_scales(i, k0 + i < k1);
+            for (int kb4 = k0; kb4 < k1 && ok; kb4 += kFar)
+#pragma unroll
+            for (int turn = 0; turn < kFar; ++turn) {
+                const int kb = kb4 + turn;
+                if (kb >= k1) break;
+                const float sw_now = sw_far[turn], row_scale = kSwap ? 0.0f : sx_far[turn] * sw_now;
+                fetch_scales(turn, kb + kFar < k1);
+                ok = __all_sync(0xffffffffu, mbar_wait(acc_full(b), bph, ctx, 24) && (!kSwap || mbar_wait(full(s), ph, ctx, 25)));
                 if (!ok) break;
                 tcgen05_fence_after();
                 const uint32_t sc = base + L.scales + s * (C::kScales * 4);
-                const float row_scale = kSwap ? 0.0f : lds_f32(sc + tl * 4) * sw_now;
                 const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + b * C::kBufCols + half * C::kPer;
-#pragma unroll
-                for (int c = 0; c < C::kPer; c += 16) {
-                    float v[16];
-                    tmem_load<16>(src + c, v);
-                    float4 sj[4];
-                    if constexpr (kSwap) {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) sj[q] = lds_f32x4(sc + (c + 4 * q) * 4);
+                auto given_back = [&]() {
+                    tcgen05_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(acc_empty(b));
+                        if constexpr (kSwap) mbar_arrive(empty(s));
                     }
-                    tmem_wait(v);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float f = kSwap ? reinterpret_cast<const float*>(sj)[j] * sw_now : row_scale;
-                        acc[c + j] = fmaf(v[j], f, acc[c + j]);
-                    }
-                }
-                tcgen05_fence_before();
-                __syncwarp();
-                if (lane == 0) { mbar_arrive(acc_empty(b)); mbar_arrive(empty(s)); }
+                };
+                if constexpr (kSwap) add_scaled_by_column(src, sc, sw_now, acc, given_back);
+                else add_scaled(src, row_scale, acc, given_back);
                 if (++s == a.stages) { s = 0; ph ^= 1; }
                 if (++b == C::kBufs) { b = 0; bph ^= 1; }
             }
@@ -332,7 +396,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                             if (x0 + j < a.m) store_one(a, x0 + j, w0 + tl, acc[j]);
                     }
                 } else if (x0 + tl < a.m) {
-                    store_run(a, x0 + tl, w0 + half * C::kPer, acc);
+                    store_run<C::kPer>(a, x0 + tl, w0 + half * C::kPer, acc);
                 }
                 continue;
             }
@@ -385,27 +449,200 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     if (a.cluster > 1) cluster_sync_all();                              // no CTA leaves while its peers still send to it
 }
 
+// ------------------------------------------------------------------- CTA pairs
+// A tile of 256 x 256 for two CTAs: 128 rows of x and half of the weight rows each, one tcgen05.mma.cta_group::2 over both (M
+// 256, N 256).  What bounds a single CTA's 128 x 256 is the way from the L2 into an SM (64 bytes a cycle): 48 KB a block, 760
+// cycles for 512 cycles of MMA; the pair's CTAs fetch 32 KB each.  The even CTA (the leader) issues; its full barriers count
+// both CTAs' bytes, its commits release stages and report buffers in both, its acc_empty counts both CTAs' epilogue warps.
+constexpr uint32_t kLeaderMask = 0xFEFFFFFFu;        // clears the CTA-rank bit of a shared::cluster address
+constexpr int kPairEpi = 8, kPairThreads = (kPairEpi + 4) * 32, kPairStages = 6, kPairBufs = 2;
+constexpr uint32_t kPairHalf = 128 * 128, kPairStage = 2 * kPairHalf, kPairBars = kPairStages * kPairStage;
+constexpr uint32_t kPairMisc = kPairBars + (2 * kPairStages + 2 * kPairBufs) * 8, kPairBytes = kPairMisc + 16 + 1024;
+constexpr uint32_t kPairInstrDesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar & kLeaderMask), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(kPairInstrDesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {     // arrives in both CTAs
+    const uint16_t mask = 3;
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"(mask) : "memory");
+}
+
+__global__ void __launch_bounds__(kPairThreads, 1)
+fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Fp8Args a) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in both CTAs
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int rank = (int)cluster_ctarank();
+    auto full = [&](int s) { return base + kPairBars + s * 8; };
+    auto empty = [&](int s) { return base + kPairBars + (kPairStages + s) * 8; };
+    auto acc_full = [&](int b) { return base + kPairBars + (2 * kPairStages + b) * 8; };
+    auto acc_empty = [&](int b) { return base + kPairBars + (2 * kPairStages + kPairBufs + b) * 8; };
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + kPairMisc + 8);
+    const WaitCtx ctx{abort_flag, a.status};
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int b = 0; b < kPairBufs; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 2 * kPairEpi); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_proxy();
+    }
+    if (warp == kPairEpi + 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + kPairMisc), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tcgen05_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + kPairMisc);
+    const int step = (int)gridDim.x / 2, first = (int)blockIdx.x / 2, blocks = a.blocks;
+
+    // 3 x 128 threads start with 168 registers each; 2 x 224 + 56 is the same sum
+    if (warp >= kPairEpi) {
+        give_registers<56>();
+        if (warp == kPairEpi && lane == 0) {
+            int s = 0, ahead = 0;
+            uint32_t ph = 0;
+            auto weights = [&](int row, int kb, int st) {
+                if (rank == 0) mbar_arrive_expect_tx(full(st), 2 * kPairStage);
+                tma_load_pair(base + st * kPairStage + kPairHalf, &map_w, full(st), kb * 128, row);
+            };
+            // the first round of stages: weights ahead of the wait for the quantizer
+            for (int item = first; item < a.items && ahead < kPairStages; item += step)
+                for (int kb = 0; kb < blocks && ahead < kPairStages; ++kb) weights(item / a.x_tiles * 256 + rank * 128, kb, ahead++);
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            bool ok = true;
+            for (int item = first; item < a.items && ok; item += step) {
+                const int wt = item / a.x_tiles, w_row = wt * 256 + rank * 128, x_row = (item - wt * a.x_tiles) * 256 + rank * 128;
+                for (int kb = 0; kb < blocks; ++kb) {
+                    if (ahead > 0) --ahead;
+                    else {
+                        ok = mbar_wait(empty(s), ph ^ 1, ctx, 31);
+                        if (!ok) break;
+                        weights(w_row, kb, s);
+                    }
+                    tma_load_pair(base + s * kPairStage, &map_x, full(s), kb * 128, x_row);
+                    if (++s == kPairStages) { s = 0; ph ^= 1; }
+                }
+            }
+        }
+        if (warp == kPairEpi + 1 && lane == 0 && rank == 0) {
+            int s = 0, b = 0;
+            uint32_t ph = 0, bph = 0;
+            bool ok = true;
+            for (int item = first; item < a.items && ok; item += step) {
+                for (int kb = 0; kb < blocks; ++kb) {
+                    ok = mbar_wait(acc_empty(b), bph ^ 1, ctx, 33) && mbar_wait(full(s), ph, ctx, 34);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    const uint64_t da = make_smem_desc(base + s * kPairStage), db = make_smem_desc(base + s * kPairStage + kPairHalf);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) umma_f8_pair(tmem + b * 256, da + 2u * k, db + 2u * k, k != 0 ? 1u : 0u);
+                    umma_commit_pair(empty(s));
+                    umma_commit_pair(acc_full(b));
+                    if (++s == kPairStages) { s = 0; ph ^= 1; }
+                    if (++b == kPairBufs) { b = 0; bph ^= 1; }
+                }
+            }
+        }
+    } else {
+        take_registers<224>();
+        asm volatile("griddepcontrol.wait;" ::: "memory");              // the scales of x are the kernel before's
+        const int quad = warp & 3, half = warp >> 2;                    // lanes 32 quad .., columns 128 half ..
+        const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + half * 128;
+        int b = 0;
+        uint32_t bph = 0;
+        bool ok = true;
+        for (int item = first; item < a.items && ok; item += step) {
+            const int wt = item / a.x_tiles, w0 = wt * 256 + half * 128;
+            const int row = (item - wt * a.x_tiles) * 256 + rank * 128 + quad * 32 + lane;
+            const float* sw = a.sw + (int64_t)min(w0 / 128, (a.n - 1) / 128) * blocks;
+            const float* sx = a.sx + min(row, a.m - 1);
+            float acc[128];
+#pragma unroll
+            for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+            constexpr int kFar = 4;                                     // scales on their way, as above
+            float sx_far[kFar], sw_far[kFar];
+            auto fetch_scales = [&](int i, bool more) {
+                if (more) {
+                    sw_far[i] = __ldg(sw);
+                    sx_far[i] = __ldcg(sx);
+                }
+                ++sw;
+                sx += a.ldsx;
+            };
+#pragma unroll
+            for (int i = 0; i < kFar; ++i) fetch_scales(i, i < blocks);
+            for (int kb4 = 0; kb4 < blocks && ok; kb4 += kFar)
+#pragma unroll
+            for (int turn = 0; turn < kFar; ++turn) {
+                const int kb = kb4 + turn;
+                if (kb >= blocks) break;
+                const float f = sx_far[turn] * sw_far[turn];
+                fetch_scales(turn, kb + kFar < blocks);
+                ok = __all_sync(0xffffffffu, mbar_wait(acc_full(b), bph, ctx, 35));
+                if (!ok) break;
+                tcgen05_fence_after();
+                add_scaled(src + b * 256, f, acc, [&]() {
+                    tcgen05_fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(acc_empty(b) & kLeaderMask) : "memory");
+                });
+                if (++b == kPairBufs) { b = 0; bph ^= 1; }
+            }
+            if (ok && row < a.m) store_run(a, row, w0, acc);
+        }
+    }
+    // Both CTAs stay until the pair is done: the leader's MMAs read the peer's shared memory, the peer arrives on its barriers.
+    tcgen05_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000ull) {}
+    }
+    cluster_sync_all();
+    if (warp == kPairEpi + 1) {
+        tcgen05_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
 // ------------------------------------------------------------------------- host side
 constexpr int kMaxDevices = 64, kMaxClusterLog = 3;
 
 // Clusters of 1, 2, 4 and 8 CTAs that the current device runs at once, asked once per device and kernel.
-template <int kCols, bool kSwap>
-int active_clusters(int (&out)[kMaxClusterLog + 1]) {
-    static std::mutex lock;
-    static int known[kMaxDevices][kMaxClusterLog + 1];
-    static bool have[kMaxDevices];
+struct ActiveClusters {
+    std::mutex lock;
+    int known[kMaxDevices][kMaxClusterLog + 1];
+    bool have[kMaxDevices];
+};
+int active_clusters(ActiveClusters& of, const void* kernel, int threads, uint32_t smem, int (&out)[kMaxClusterLog + 1]) {
     int dev = 0;
     MIXFP4_CUDA_CHECK(cudaGetDevice(&dev));
     if (dev < 0 || dev >= kMaxDevices) return MIXFP4_E_UNSUPPORTED;
-    std::lock_guard<std::mutex> guard(lock);
-    if (!have[dev]) {
-        const auto kernel = fp8_gemm_kernel<kCols, kSwap>;
-        MIXFP4_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax));
+    std::lock_guard<std::mutex> guard(of.lock);
+    if (!of.have[dev]) {
+        MIXFP4_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         for (int c = 0; c <= kMaxClusterLog; ++c) {
             cudaLaunchConfig_t cfg = {};
             cfg.gridDim = dim3(1u << c);
-            cfg.blockDim = dim3(Fp8Cfg<kCols, kSwap>::kThreads);
-            cfg.dynamicSmemBytes = kSmemMax;
+            cfg.blockDim = dim3((unsigned)threads);
+            cfg.dynamicSmemBytes = smem;
             cudaLaunchAttribute attr[1];
             attr[0].id = cudaLaunchAttributeClusterDimension;
             attr[0].val.clusterDim.x = 1u << c;
@@ -417,11 +654,11 @@ int active_clusters(int (&out)[kMaxClusterLog + 1]) {
                 (void)cudaGetLastError();                               // a cluster size the device does not take
                 n = 0;
             }
-            known[dev][c] = n;
+            of.known[dev][c] = n;
         }
-        have[dev] = true;
+        of.have[dev] = true;
     }
-    for (int c = 0; c <= kMaxClusterLog; ++c) out[c] = known[dev][c];
+    for (int c = 0; c <= kMaxClusterLog; ++c) out[c] = of.known[dev][c];
     return MIXFP4_OK;
 }
 
@@ -442,70 +679,85 @@ int encode_codes(EncodeTiledFn fn, CUtensorMap* map, const uint8_t* p, int64_t r
     return r == CUDA_SUCCESS ? MIXFP4_OK : record_error_text("cuTensorMapEncodeTiled failed for an fp8 operand");
 }
 
-// Microseconds that an arrangement would take: rounds of items times blocks in a run.  Per block: what the weights of one SM
+struct Fp8Choice {
+    float cost = 1e30f;
+    int cols = 0, cluster_log = 0, active = 0;
+};
+// An arrangement's cost in microseconds: rounds of items times blocks of K in a run.  Per block: what the weights of one SM
 // take from HBM, or the tensor core and the epilogue; per item: filling and draining the pipeline, an exchange.
 template <int kCols, bool kSwap>
-float fp8_cost(const Fp8Args& a, int cluster_log, const int* clusters) {
-    const int c = 1 << cluster_log;
-    if (clusters[cluster_log] < 1 || c > a.blocks || (kCols > 128 && c > 1)) return 1e30f;
+int consider(const Fp8Args& a, Fp8Choice& best) {
+    static ActiveClusters active;
+    int clusters[kMaxClusterLog + 1];
+    const auto kernel = fp8_gemm_kernel<kCols, kSwap>;
+    if (const int rc = active_clusters(active, reinterpret_cast<const void*>(kernel), Fp8Cfg<kCols, kSwap>::kThreads, kSmemMax, clusters))
+        return rc;
     const int64_t lanes = kSwap ? a.n : a.m, cols = kSwap ? a.m : a.n;
     const int64_t items = (lanes + 127) / 128 * ((cols + kCols - 1) / kCols);
-    const int64_t rounds = (items + clusters[cluster_log] - 1) / clusters[cluster_log];
-    const float block = kSwap ? 0.38f : kCols == 128 ? 0.24f : 0.36f;
-    return (float)rounds * (block * (float)((a.blocks + c - 1) / c) + (c > 1 ? 1.5f : 0.7f));
+    for (int log = 0; log <= kMaxClusterLog; ++log) {
+        const int c = 1 << log;
+        if (clusters[log] < 1 || c > a.blocks) continue;
+        const int64_t rounds = (items + clusters[log] - 1) / clusters[log];
+        const float block = kSwap ? 0.38f : 0.30f;
+        const float cost = (float)rounds * (block * (float)((a.blocks + c - 1) / c) + (c > 1 ? 1.5f : 0.7f));
+        if (cost < best.cost) best = Fp8Choice{cost, kCols, log, clusters[log]};
+    }
+    return MIXFP4_OK;
+}
+int consider_pair(const Fp8Args& a, Fp8Choice& best) {
+    static ActiveClusters active;
+    int clusters[kMaxClusterLog + 1];
+    if (const int rc = active_clusters(active, reinterpret_cast<const void*>(fp8_pair_kernel), kPairThreads, kPairBytes, clusters)) return rc;
+    if (clusters[1] < 1) return MIXFP4_OK;
+    const int64_t items = (int64_t)((a.m + 255) / 256) * ((a.n + 255) / 256), rounds = (items + clusters[1] - 1) / clusters[1];
+    const float cost = (float)rounds * (0.36f * (float)a.blocks + 1.5f);
+    if (cost < best.cost) best = Fp8Choice{cost, 256, 1, clusters[1]};
+    return MIXFP4_OK;
 }
 
-template <int kCols, bool kSwap>
-int launch_fp8(Fp8Args a, const Fp8Problem& p, int cluster_log, const int* clusters, cudaStream_t st) {
-    using C = Fp8Cfg<kCols, kSwap>;
-    EncodeTiledFn fn = encode_tiled_fn();
-    if (!fn) return record_error_text("cuTensorMapEncodeTiled is not available");
-    CUtensorMap map_x, map_w;
-    if (const int rc = encode_codes(fn, &map_x, p.x, a.m, p.k, p.ldx, kSwap ? kCols : 128)) return rc;
-    if (const int rc = encode_codes(fn, &map_w, p.w, a.n, p.k, p.ldw, kSwap ? 128 : kCols)) return rc;
-    a.cluster = 1 << cluster_log;
-    a.x_tiles = (a.m + (kSwap ? kCols : 128) - 1) / (kSwap ? kCols : 128);
-    const int64_t items = (int64_t)a.x_tiles * ((a.n + (kSwap ? 128 : kCols) - 1) / (kSwap ? 128 : kCols));
-    if (items > 0x3fffffff) return MIXFP4_E_SHAPE;
-    a.items = (int)items;
-    a.stages = kMaxStages;
-    while (fp8_layout<kCols, kSwap>(a.stages, a.cluster).bytes > kSmemMax) --a.stages;
-    const int n = a.items < clusters[cluster_log] ? a.items : clusters[cluster_log];
+int launch_clusters(const void* kernel, int cluster, int n, int threads, uint32_t smem, const Fp8Problem& p, const CUtensorMap& map_x,
+                    const CUtensorMap& map_w, const Fp8Args& a, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(n * a.cluster));
-    cfg.blockDim = dim3(C::kThreads);
-    cfg.dynamicSmemBytes = fp8_layout<kCols, kSwap>(a.stages, a.cluster).bytes;
+    cfg.gridDim = dim3((unsigned)(n * cluster));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)a.cluster;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.dependent ? 2 : 1;
-    const auto kernel = fp8_gemm_kernel<kCols, kSwap>;
-    MIXFP4_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, map_x, map_w, a));
-    return check_launch("fp8_gemm_kernel");
+    void* args[] = {const_cast<CUtensorMap*>(&map_x), const_cast<CUtensorMap*>(&map_w), const_cast<Fp8Args*>(&a)};
+    MIXFP4_CUDA_CHECK(cudaLaunchKernelExC(&cfg, kernel, args));
+    return check_launch("fp8 product");
 }
 
-struct Fp8Choice {
-    float cost = 1e30f;
-    int cols = 0, cluster_log = 0;
-    int clusters[kMaxClusterLog + 1] = {};
-};
+// Maps with boxes of x_box rows of x and w_box rows of the weight; items of `tile` rows each.
+int launch_fp8(Fp8Args a, const Fp8Problem& p, const Fp8Choice& c, int x_box, int w_box, int x_tile, int w_tile, const void* kernel,
+               int threads, uint32_t smem, cudaStream_t st) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return record_error_text("cuTensorMapEncodeTiled is not available");
+    CUtensorMap map_x, map_w;
+    if (const int rc = encode_codes(fn, &map_x, p.x, a.m, p.k, p.ldx, (uint32_t)x_box)) return rc;
+    if (const int rc = encode_codes(fn, &map_w, p.w, a.n, p.k, p.ldw, (uint32_t)w_box)) return rc;
+    a.x_tiles = (a.m + x_tile - 1) / x_tile;
+    const int64_t items = (int64_t)a.x_tiles * ((a.n + w_tile - 1) / w_tile);
+    if (items > 0x3fffffff) return MIXFP4_E_SHAPE;
+    a.items = (int)items;
+    return launch_clusters(kernel, 1 << c.cluster_log, a.items < c.active ? a.items : c.active, threads, smem, p, map_x, map_w, a, st);
+}
 template <int kCols, bool kSwap>
-int consider(const Fp8Args& a, Fp8Choice& best) {
-    int clusters[kMaxClusterLog + 1];
-    if (const int rc = active_clusters<kCols, kSwap>(clusters)) return rc;
-    for (int c = 0; c <= kMaxClusterLog; ++c) {
-        const float t = fp8_cost<kCols, kSwap>(a, c, clusters);
-        if (t < best.cost) {
-            best.cost = t; best.cols = kCols; best.cluster_log = c;
-            for (int i = 0; i <= kMaxClusterLog; ++i) best.clusters[i] = clusters[i];
-        }
-    }
-    return MIXFP4_OK;
+int launch_single(Fp8Args a, const Fp8Problem& p, const Fp8Choice& c, cudaStream_t st) {
+    a.cluster = 1 << c.cluster_log;
+    a.stages = kMaxStages;
+    while (fp8_layout<kCols, kSwap>(a.stages, a.cluster).bytes > kSmemMax) --a.stages;
+    const auto kernel = fp8_gemm_kernel<kCols, kSwap>;
+    constexpr int kX = kSwap ? kCols : 128, kW = kSwap ? 128 : kCols;
+    return launch_fp8(a, p, c, kX, kW, kX, kW, reinterpret_cast<const void*>(kernel), Fp8Cfg<kCols, kSwap>::kThreads,
+                      fp8_layout<kCols, kSwap>(a.stages, a.cluster).bytes, st);
 }
 
 int fp8_gemm(const Fp8Args& a, const Fp8Problem& p, cudaStream_t st) {
@@ -514,14 +766,14 @@ int fp8_gemm(const Fp8Args& a, const Fp8Problem& p, cudaStream_t st) {
     if (a.m <= 16) rc = consider<16, true>(a, best);
     else if (a.m <= 32) rc = consider<32, true>(a, best);
     else if (a.m <= 64) rc = consider<64, true>(a, best);
-    else if (!(rc = consider<128, false>(a, best))) rc = consider<256, false>(a, best);
+    else if (!(rc = consider<128, false>(a, best))) rc = consider_pair(a, best);
     if (rc) return rc;
     switch (best.cols) {
-        case 16: return launch_fp8<16, true>(a, p, best.cluster_log, best.clusters, st);
-        case 32: return launch_fp8<32, true>(a, p, best.cluster_log, best.clusters, st);
-        case 64: return launch_fp8<64, true>(a, p, best.cluster_log, best.clusters, st);
-        case 128: return launch_fp8<128, false>(a, p, best.cluster_log, best.clusters, st);
-        case 256: return launch_fp8<256, false>(a, p, best.cluster_log, best.clusters, st);
+        case 16: return launch_single<16, true>(a, p, best, st);
+        case 32: return launch_single<32, true>(a, p, best, st);
+        case 64: return launch_single<64, true>(a, p, best, st);
+        case 128: return launch_single<128, false>(a, p, best, st);
+        case 256: return launch_fp8(a, p, best, 128, 128, 256, 256, reinterpret_cast<const void*>(fp8_pair_kernel), kPairThreads, kPairBytes, st);
         default: return MIXFP4_E_UNSUPPORTED;
     }
 }
@@ -543,7 +795,7 @@ Fp8Args make_args(const float* sx, int64_t ldsx, const float* sw, int64_t m, int
     a.sx = sx; a.sw = sw; a.y = y; a.ldsx = ldsx; a.ldy = ldy;
     a.m = (int)m; a.n = (int)n; a.blocks = (int)((k + kFp8Block - 1) / kFp8Block);
     a.out_dtype = out_dtype; a.status = status;
-    a.y_vec = aligned(y, 16) && ldy * (out_dtype == MIXFP4_F32 ? 4 : 2) % 16 == 0;
+    a.y_vec = aligned(y, 32) && ldy * (out_dtype == MIXFP4_F32 ? 4 : 2) % 32 == 0;
     return a;
 }
 
