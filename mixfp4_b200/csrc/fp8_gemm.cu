@@ -71,17 +71,47 @@ __host__ __device__ inline Fp8Layout fp8_layout(int stages, int cluster) {
     return l;
 }
 
-__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
+// The single-warp roles run converged, and their issuing instructions take the elected lane as a predicate: the code around
+// them stays uniform, their operands in uniform registers.  (A branch for one lane took three times as long a block.)
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p;
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const WaitCtx& ctx, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, ctx, code));
+}
+__device__ __forceinline__ void expect_if(uint32_t lead, uint32_t bar, uint32_t bytes) {
+    asm volatile(
+        "{\n\t.reg .pred l;\n\tsetp.ne.u32 l, %0, 0;\n\t"
+        "@l mbarrier.arrive.expect_tx.shared::cta.b64 _, [%1], %2;\n\t}"
+        ::"r"(lead), "r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_load_if(uint32_t lead, uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "{\n\t.reg .pred l;\n\tsetp.ne.u32 l, %0, 0;\n\t"
+        "@l cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%2, {%4, %5}], [%3];\n\t}"
+        ::"r"(lead), "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void bulk_load_if(uint32_t lead, uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred l;\n\tsetp.ne.u32 l, %0, 0;\n\t"
+        "@l cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%2], %3, [%4];\n\t}"
+        ::"r"(lead), "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void umma_f8_if(uint32_t lead, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, l;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\tsetp.ne.u32 l, %0, 0;\n\t"
+        "@l tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], %2, %3, %4, p;\n\t}"
+        ::"r"(lead), "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_commit_if(uint32_t lead, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred l;\n\tsetp.ne.u32 l, %0, 0;\n\t"
+        "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}"
+        ::"r"(lead), "r"(bar) : "memory");
 }
 // 16 or 32 columns of this warp's 32 lanes, without the wait.
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
@@ -282,55 +312,54 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     const int k0 = a.blocks * rank / a.cluster, k1 = a.blocks * (rank + 1) / a.cluster;
     const int step = (int)gridDim.x / a.cluster, first = (int)blockIdx.x / a.cluster;
 
-    if (warp >= C::kEpi) {
-        if (warp == C::kEpi && lane == 0) {
-            // Weights never depend on the kernel before (the quantizer of x): the first round of stages asks for them ahead of the wait.
-            int s = 0, ahead = 0;
-            uint32_t ph = 0;
-            auto weights = [&](int item, int kb, int st) {
-                mbar_arrive_expect_tx(full(st), C::kStage + C::kScales * 4);
-                const uint32_t dst = base + st * C::kStage + (kSwap ? 0u : C::kABytes);
-                tma_load_2d(dst, &map_w, full(st), kb * 128, item / a.x_tiles * (kSwap ? 128 : kCols));
-            };
-            for (int item = first; item < a.items && ahead < a.stages; item += step)
-                for (int kb = k0; kb < k1 && ahead < a.stages; ++kb) weights(item, kb, ahead++);
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            asm volatile("fence.proxy.async.global;" ::: "memory");     // ordinary stores of that kernel, read by TMA
-            bool ok = true;
-            for (int item = first; item < a.items && ok; item += step) {
-                const int x0 = item % a.x_tiles * (kSwap ? kCols : 128);
-                for (int kb = k0; kb < k1; ++kb) {
-                    if (ahead > 0) --ahead;
-                    else {
-                        ok = mbar_wait(empty(s), ph ^ 1, ctx, 21);
-                        if (!ok) break;
-                        weights(item, kb, s);
-                    }
-                    tma_load_2d(base + s * C::kStage + (kSwap ? C::kABytes : 0u), &map_x, full(s), kb * 128, x0);
-                    if constexpr (kSwap)
-                        bulk_load(base + L.scales + s * (C::kScales * 4), a.sx + (int64_t)kb * a.ldsx + x0, C::kScales * 4, full(s));
-                    if (++s == a.stages) { s = 0; ph ^= 1; }
+    if (warp == C::kEpi) {
+        // Weights never depend on the kernel before (the quantizer of x): the first round of stages asks for them ahead of the wait.
+        const uint32_t lead = elect_one();
+        int s = 0, ahead = 0;
+        uint32_t ph = 0;
+        auto weights = [&](int row, int kb, int st) {
+            expect_if(lead, full(st), C::kStage + C::kScales * 4);
+            tma_load_if(lead, base + st * C::kStage + (kSwap ? 0u : C::kABytes), &map_w, full(st), kb * 128, row);
+        };
+        for (int item = first; item < a.items && ahead < a.stages; item += step)
+            for (int kb = k0; kb < k1 && ahead < a.stages; ++kb) weights(item / a.x_tiles * (kSwap ? 128 : kCols), kb, ahead++);
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("fence.proxy.async.global;" ::: "memory");         // ordinary stores of that kernel, read by TMA
+        bool ok = true;
+        for (int item = first; item < a.items && ok; item += step) {
+            const int wt = item / a.x_tiles, w_row = wt * (kSwap ? 128 : kCols), x_row = (item - wt * a.x_tiles) * (kSwap ? kCols : 128);
+            for (int kb = k0; kb < k1; ++kb) {
+                if (ahead > 0) --ahead;
+                else {
+                    ok = warp_wait(empty(s), ph ^ 1, ctx, 21);
+                    if (!ok) break;
+                    weights(w_row, kb, s);
                 }
+                tma_load_if(lead, base + s * C::kStage + (kSwap ? C::kABytes : 0u), &map_x, full(s), kb * 128, x_row);
+                if constexpr (kSwap)
+                    bulk_load_if(lead, base + L.scales + s * (C::kScales * 4), a.sx + (int64_t)kb * a.ldsx + x_row, C::kScales * 4, full(s));
+                if (++s == a.stages) { s = 0; ph ^= 1; }
             }
         }
-        if (warp == C::kEpi + 1 && lane == 0) {
-            int s = 0, b = 0;
-            uint32_t ph = 0, bph = 0;
-            bool ok = true;
-            for (int item = first; item < a.items && ok; item += step) {
-                for (int kb = k0; kb < k1; ++kb) {
-                    ok = mbar_wait(acc_empty(b), bph ^ 1, ctx, 22) && mbar_wait(full(s), ph, ctx, 23);
-                    if (!ok) break;
-                    tcgen05_fence_after();
-                    const uint64_t da = make_smem_desc(base + s * C::kStage), db = make_smem_desc(base + s * C::kStage + C::kABytes);
+    } else if (warp == C::kEpi + 1) {
+        const uint32_t lead = elect_one();
+        const uint64_t a_desc = make_smem_desc(base), b_desc = make_smem_desc(base + C::kABytes);
+        int s = 0, b = 0;
+        uint32_t ph = 0, bph = 0;
+        bool ok = true;
+        for (int item = first; item < a.items && ok; item += step) {
+            for (int kb = k0; kb < k1; ++kb) {
+                ok = warp_wait(full(s), ph, ctx, 23) && warp_wait(acc_empty(b), bph ^ 1, ctx, 22);
+                if (!ok) break;
+                tcgen05_fence_after();
+                const uint64_t at = (uint64_t)(s * (C::kStage >> 4));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_f8(tmem + b * C::kBufCols, da + 2u * k, db + 2u * k, C::kInstrDesc, k != 0 ? 1u : 0u);
-                    umma_commit(empty(s));
-                    umma_commit(acc_full(b));
-                    if (++s == a.stages) { s = 0; ph ^= 1; }
-                    if (++b == C::kBufs) { b = 0; bph ^= 1; }
-                }
+                for (int k = 0; k < 4; ++k)
+                    umma_f8_if(lead, tmem + b * C::kBufCols, a_desc + at + 2u * k, b_desc + at + 2u * k, C::kInstrDesc, k != 0 ? 1u : 0u);
+                umma_commit_if(lead, empty(s));
+                umma_commit_if(lead, acc_full(b));
+                if (++s == a.stages) { s = 0; ph ^= 1; }
+                if (++b == C::kBufs) { b = 0; bph ^= 1; }
             }
         }
     } else {
@@ -460,22 +489,25 @@ constexpr uint32_t kPairHalf = 128 * 128, kPairStage = 2 * kPairHalf, kPairBars 
 constexpr uint32_t kPairMisc = kPairBars + (2 * kPairStages + 2 * kPairBufs) * 8, kPairBytes = kPairMisc + 16 + 1024;
 constexpr uint32_t kPairInstrDesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
 
-__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+__device__ __forceinline__ void tma_load_pair_if(uint32_t lead, uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar & kLeaderMask), "r"(c0), "r"(c1) : "memory");
+        "{\n\t.reg .pred l;\n\tsetp.ne.u32 l, %0, 0;\n\t"
+        "@l cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%2, {%4, %5}], [%3];\n\t}"
+        ::"r"(lead), "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar & kLeaderMask), "r"(c0), "r"(c1) : "memory");
 }
-__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_f8_pair_if(uint32_t lead, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(kPairInstrDesc), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred p, l;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\tsetp.ne.u32 l, %0, 0;\n\t"
+        "@l tcgen05.mma.cta_group::2.kind::f8f6f4 [%1], %2, %3, %4, p;\n\t}"
+        ::"r"(lead), "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(kPairInstrDesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {     // arrives in both CTAs
+__device__ __forceinline__ void umma_commit_pair_if(uint32_t lead, uint32_t bar) {     // arrives in both CTAs
     const uint16_t mask = 3;
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar), "h"(mask) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred l;\n\tsetp.ne.u32 l, %0, 0;\n\t"
+        "@l tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%1], %2;\n\t}"
+        ::"r"(lead), "r"(bar), "h"(mask) : "memory");
 }
 
 __global__ void __launch_bounds__(kPairThreads, 1)
@@ -513,12 +545,13 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     // 3 x 128 threads start with 168 registers each; 2 x 224 + 56 is the same sum
     if (warp >= kPairEpi) {
         give_registers<56>();
-        if (warp == kPairEpi && lane == 0) {
+        if (warp == kPairEpi) {
+            const uint32_t lead = elect_one(), lead0 = rank == 0 ? lead : 0u;
             int s = 0, ahead = 0;
             uint32_t ph = 0;
             auto weights = [&](int row, int kb, int st) {
-                if (rank == 0) mbar_arrive_expect_tx(full(st), 2 * kPairStage);
-                tma_load_pair(base + st * kPairStage + kPairHalf, &map_w, full(st), kb * 128, row);
+                expect_if(lead0, full(st), 2 * kPairStage);
+                tma_load_pair_if(lead, base + st * kPairStage + kPairHalf, &map_w, full(st), kb * 128, row);
             };
             // the first round of stages: weights ahead of the wait for the quantizer
             for (int item = first; item < a.items && ahead < kPairStages; item += step)
@@ -531,29 +564,31 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 for (int kb = 0; kb < blocks; ++kb) {
                     if (ahead > 0) --ahead;
                     else {
-                        ok = mbar_wait(empty(s), ph ^ 1, ctx, 31);
+                        ok = warp_wait(empty(s), ph ^ 1, ctx, 31);
                         if (!ok) break;
                         weights(w_row, kb, s);
                     }
-                    tma_load_pair(base + s * kPairStage, &map_x, full(s), kb * 128, x_row);
+                    tma_load_pair_if(lead, base + s * kPairStage, &map_x, full(s), kb * 128, x_row);
                     if (++s == kPairStages) { s = 0; ph ^= 1; }
                 }
             }
-        }
-        if (warp == kPairEpi + 1 && lane == 0 && rank == 0) {
+        } else if (warp == kPairEpi + 1 && rank == 0) {
+            const uint32_t lead = elect_one();
+            const uint64_t a_desc = make_smem_desc(base), b_desc = make_smem_desc(base + kPairHalf);
             int s = 0, b = 0;
             uint32_t ph = 0, bph = 0;
             bool ok = true;
             for (int item = first; item < a.items && ok; item += step) {
                 for (int kb = 0; kb < blocks; ++kb) {
-                    ok = mbar_wait(acc_empty(b), bph ^ 1, ctx, 33) && mbar_wait(full(s), ph, ctx, 34);
+                    ok = warp_wait(full(s), ph, ctx, 34) && warp_wait(acc_empty(b), bph ^ 1, ctx, 33);
                     if (!ok) break;
                     tcgen05_fence_after();
-                    const uint64_t da = make_smem_desc(base + s * kPairStage), db = make_smem_desc(base + s * kPairStage + kPairHalf);
+                    const uint64_t at = (uint64_t)(s * (kPairStage >> 4));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) umma_f8_pair(tmem + b * 256, da + 2u * k, db + 2u * k, k != 0 ? 1u : 0u);
-                    umma_commit_pair(empty(s));
-                    umma_commit_pair(acc_full(b));
+                    for (int k = 0; k < 4; ++k)
+                        umma_f8_pair_if(lead, tmem + b * 256, a_desc + at + 2u * k, b_desc + at + 2u * k, k != 0 ? 1u : 0u);
+                    umma_commit_pair_if(lead, empty(s));
+                    umma_commit_pair_if(lead, acc_full(b));
                     if (++s == kPairStages) { s = 0; ph ^= 1; }
                     if (++b == kPairBufs) { b = 0; bph ^= 1; }
                 }
