@@ -413,7 +413,8 @@ MIXFP4_API int mixfp4_fp8_dequant(const uint8_t* codes, int64_t ldq, const float
  * multiples of 16; what lies behind k in a row is not read.  x_scales as mixfp4_fp8_quantize_rows lays them out (the pad rows
  * are read, their values do not matter).  status as in mixfp4_gemm.
  * mixfp4_fp8_linear: the same with x still dense: quantized into the workspace (at least
- * mixfp4_fp8_workspace_bytes(m, k) bytes, 16-byte aligned), then multiplied, the product starting under the quantizer's tail. */
+ * mixfp4_fp8_workspace_bytes(m, k) bytes, 16-byte aligned), then multiplied, the product starting under the quantizer's tail.
+ * Few rows of a short K are quantized by the product itself: no workspace (0 bytes), one launch, the same bits. */
 MIXFP4_API int mixfp4_fp8_gemm(const uint8_t* x, int64_t ldx, const float* x_scales, int64_t lds, const uint8_t* w,
                     int64_t ldw, const float* w_scales, int64_t m, int64_t n, int64_t k, void* y, int out_dtype,
                     int64_t ldy, int* status, void* stream);

@@ -32,23 +32,28 @@ constexpr int kMaxStages = 12;
 constexpr uint32_t kSmemMax = 227 * 1024;
 
 struct Fp8Args {
+    const void* x;                       // dense rows, where the kernel quantizes them itself
+    int64_t ldx;
+    int x_dtype;
+    bool x_vec;
     const float* sx;                     // [blocks][ldsx]
     const float* sw;                     // [ceil(n / 128)][blocks]
     void* y;
     int64_t ldsx, ldy;
-    int m, n, blocks;
+    int m, n, k, blocks;
     int x_tiles, items, cluster, stages, out_dtype;
     bool y_vec;                          // rows of y are 32-byte aligned
     int* status;
 };
 
-template <int kCols, bool kSwap>
+// kOwn: x is dense and quantized by every CTA, its run of K for all rows, into shared memory.
+template <int kCols, bool kSwap, bool kOwn>
 struct Fp8Cfg {
     static constexpr int kEpi = kCols > 64 ? 8 : 4;                     // epilogue warps: 64 columns a thread at most
     static constexpr int kPer = kCols * 4 / kEpi;                       // columns of a thread
     static constexpr int kThreads = (kEpi + 2) * 32;
-    static constexpr uint32_t kABytes = 128 * 128, kBBytes = kCols * 128, kStage = kABytes + kBBytes;
-    static constexpr int kScales = kSwap ? kCols : 0;                   // scales of x in a stage
+    static constexpr uint32_t kABytes = 128 * 128, kBBytes = kCols * 128, kStage = kABytes + (kOwn ? 0 : kBBytes);
+    static constexpr int kScales = kSwap && !kOwn ? kCols : 0;          // scales of x in a stage
     static constexpr int kBufs = 4;
     static constexpr uint32_t kBufCols = kCols < 32 ? 32 : kCols, kTmemCols = kBufs * kBufCols;
     // D fp32, A and B E4M3, both K-major
@@ -57,17 +62,20 @@ struct Fp8Cfg {
 };
 
 struct Fp8Layout {
-    uint32_t scales, exchange, bars, misc, bytes;
+    uint32_t own, own_scales, scales, exchange, bars, misc, bytes;
 };
-template <int kCols, bool kSwap>
-__host__ __device__ inline Fp8Layout fp8_layout(int stages, int cluster) {
-    using C = Fp8Cfg<kCols, kSwap>;
+template <int kCols, bool kSwap, bool kOwn>
+__host__ __device__ inline Fp8Layout fp8_layout(int stages, int cluster, int blocks) {
+    using C = Fp8Cfg<kCols, kSwap, kOwn>;
+    const uint32_t run = kOwn ? (uint32_t)((blocks + cluster - 1) / cluster) : 0u;
     Fp8Layout l;
-    l.scales = (uint32_t)stages * C::kStage;
+    l.own = (uint32_t)stages * C::kStage;
+    l.own_scales = l.own + run * C::kBBytes;
+    l.scales = l.own_scales + run * kCols * 4u;
     l.exchange = l.scales + (uint32_t)stages * C::kScales * 4u;
     l.bars = l.exchange + (cluster > 1 ? 128u * C::kPitch * 4u : 0u);
-    l.misc = l.bars + (2 * kMaxStages + 2 * 4 + 2) * 8;
-    l.bytes = l.misc + 16 + 1024;                                       // + alignment slack
+    l.misc = l.bars + (2 * kMaxStages + 2 * 4 + 3) * 8;
+    l.bytes = (l.misc + 16 + 1024 + 7) & ~7u;                           // + alignment slack
     return l;
 }
 
@@ -274,29 +282,63 @@ __device__ __forceinline__ void add_scaled_by_column(uint32_t src, uint32_t sc, 
     }
 }
 
-template <int kCols, bool kSwap>
-__global__ void __launch_bounds__(Fp8Cfg<kCols, kSwap>::kThreads, 1)
+// Rows of x and blocks k0 .. k1 of K: codes as the B operand of the product (kCols rows of 128 bytes a block, swizzled), scales
+// as [block][kCols].  Rows that x does not have stay as they are: they make columns that nobody stores.  A group of eight lanes
+// takes four blocks at a time, all loads before the first is used.
+template <int kCols, typename T>
+__device__ __forceinline__ void quantize_own(const Fp8Args& a, uint8_t* codes, float* scales, int k0, int k1, int thread, int threads) {
+    constexpr int kAhead = 4;
+    const T* x = static_cast<const T*>(a.x);
+    const int sub = thread % kLanesPerRow, groups = (k1 - k0) * a.m, step = threads / kLanesPerRow;
+    for (int first = 0; first < groups; first += kAhead * step) {
+        Raw<T> v[kAhead];
+        int block[kAhead], row[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int g = first + i * step + thread / kLanesPerRow;
+            block[i] = g / a.m;
+            row[i] = g - block[i] * a.m;
+            load16(x + row[i] * a.ldx, (int64_t)(k0 + block[i]) * kFp8Block + sub * kLaneElems, g < groups ? a.k : 0, a.x_vec, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            uint32_t most = largest_of(v[i]);
+#pragma unroll
+            for (int d = 1; d < kLanesPerRow; d *= 2) most = larger<T>(most, __shfl_xor_sync(0xffffffffu, most, d));
+            if (first + i * step + thread / kLanesPerRow >= groups) continue;
+            const float s = block_scale(magnitude<T>(most));
+            const int at = block[i] * kCols + row[i];
+            *reinterpret_cast<uint4*>(codes + at * 128 + ((sub ^ (row[i] & 7)) * 16)) = encode16(v[i], s);
+            if (sub == 0) scales[at] = s;
+        }
+    }
+}
+
+template <int kCols, bool kSwap, bool kOwn>
+__global__ void __launch_bounds__(Fp8Cfg<kCols, kSwap, kOwn>::kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Fp8Args a) {
-    using C = Fp8Cfg<kCols, kSwap>;
+    using C = Fp8Cfg<kCols, kSwap, kOwn>;
+    constexpr bool kRingScales = kSwap && !kOwn;                        // a stage holds scales of x: it waits for the epilogue
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in every CTA of the cluster
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    const Fp8Layout L = fp8_layout<kCols, kSwap>(a.stages, a.cluster);
+    const Fp8Layout L = fp8_layout<kCols, kSwap, kOwn>(a.stages, a.cluster, a.blocks);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int rank = (int)cluster_ctarank();
     auto full = [&](int s) { return base + L.bars + s * 8; };
     auto empty = [&](int s) { return base + L.bars + (kMaxStages + s) * 8; };
     auto acc_full = [&](int b) { return base + L.bars + (2 * kMaxStages + b) * 8; };
     auto acc_empty = [&](int b) { return base + L.bars + (2 * kMaxStages + 4 + b) * 8; };
-    const uint32_t sums_in = base + L.bars + (2 * kMaxStages + 8) * 8, sums_out = sums_in + 8;
+    const uint32_t sums_in = base + L.bars + (2 * kMaxStages + 8) * 8, sums_out = sums_in + 8, x_ready = sums_in + 16;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen + L.misc + 8);
     const WaitCtx ctx{abort_flag, a.status};
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < a.stages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), kSwap ? 1 + C::kEpi : 1); }
+        for (int s = 0; s < a.stages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), kRingScales ? 1 + C::kEpi : 1); }
         for (int b = 0; b < C::kBufs; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), C::kEpi); }
         mbar_init(sums_in, (uint32_t)a.cluster * C::kEpi);              // every warp of every CTA of the cluster has sent
         mbar_init(sums_out, (uint32_t)a.cluster * C::kEpi);             // ... and has added its share of what was sent
+        if constexpr (kOwn) mbar_init(x_ready, C::kEpi);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_proxy();
@@ -335,27 +377,28 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     if (!ok) break;
                     weights(w_row, kb, s);
                 }
-                tma_load_if(lead, base + s * C::kStage + (kSwap ? C::kABytes : 0u), &map_x, full(s), kb * 128, x_row);
-                if constexpr (kSwap)
+                if constexpr (!kOwn) tma_load_if(lead, base + s * C::kStage + (kSwap ? C::kABytes : 0u), &map_x, full(s), kb * 128, x_row);
+                if constexpr (kRingScales)
                     bulk_load_if(lead, base + L.scales + s * (C::kScales * 4), a.sx + (int64_t)kb * a.ldsx + x_row, C::kScales * 4, full(s));
                 if (++s == a.stages) { s = 0; ph ^= 1; }
             }
         }
     } else if (warp == C::kEpi + 1) {
         const uint32_t lead = elect_one();
-        const uint64_t a_desc = make_smem_desc(base), b_desc = make_smem_desc(base + C::kABytes);
+        const uint64_t a_desc = make_smem_desc(base), b_desc = make_smem_desc(base + (kOwn ? L.own : C::kABytes));
         int s = 0, b = 0;
         uint32_t ph = 0, bph = 0;
         bool ok = true;
+        if constexpr (kOwn) ok = warp_wait(x_ready, 0, ctx, 20);
         for (int item = first; item < a.items && ok; item += step) {
             for (int kb = k0; kb < k1; ++kb) {
                 ok = warp_wait(full(s), ph, ctx, 23) && warp_wait(acc_empty(b), bph ^ 1, ctx, 22);
                 if (!ok) break;
                 tcgen05_fence_after();
-                const uint64_t at = (uint64_t)(s * (C::kStage >> 4));
+                const uint64_t at = (uint64_t)(s * (C::kStage >> 4)), b_at = kOwn ? (uint64_t)((kb - k0) * (C::kBBytes >> 4)) : at;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    umma_f8_if(lead, tmem + b * C::kBufCols, a_desc + at + 2u * k, b_desc + at + 2u * k, C::kInstrDesc, k != 0 ? 1u : 0u);
+                    umma_f8_if(lead, tmem + b * C::kBufCols, a_desc + at + 2u * k, b_desc + b_at + 2u * k, C::kInstrDesc, k != 0 ? 1u : 0u);
                 umma_commit_if(lead, empty(s));
                 umma_commit_if(lead, acc_full(b));
                 if (++s == a.stages) { s = 0; ph ^= 1; }
@@ -366,6 +409,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         if constexpr (!kSwap) asm volatile("griddepcontrol.wait;" ::: "memory");     // the scales are the kernel before's
         const int quad = warp & 3, half = warp >> 2;                    // lanes 32 quad .., columns half * kPer ..
         const int tl = quad * 32 + lane;
+        if constexpr (kOwn) {
+            uint8_t* codes = gen + L.own;
+            float* scales = reinterpret_cast<float*>(gen + L.own_scales);
+            if (a.x_dtype == MIXFP4_BF16) quantize_own<kCols, __nv_bfloat16>(a, codes, scales, k0, k1, threadIdx.x, C::kEpi * 32);
+            else if (a.x_dtype == MIXFP4_F16) quantize_own<kCols, __half>(a, codes, scales, k0, k1, threadIdx.x, C::kEpi * 32);
+            else quantize_own<kCols, float>(a, codes, scales, k0, k1, threadIdx.x, C::kEpi * 32);
+            fence_async_proxy();                                        // the tensor core reads the codes
+            __syncwarp();
+            if (lane == 0) mbar_arrive(x_ready);
+            mbar_wait(x_ready, 0, ctx, 28);                             // the other warps' scales; what expires shows below
+        }
         int s = 0, b = 0;
         uint32_t ph = 0, bph = 0, xph = 0;
         bool ok = true;
@@ -398,17 +452,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 if (kb >= k1) break;
                 const float sw_now = sw_far[turn], row_scale = kSwap ? 0.0f : sx_far[turn] * sw_now;
                 fetch_scales(turn, kb + kFar < k1);
-                ok = __all_sync(0xffffffffu, mbar_wait(acc_full(b), bph, ctx, 24) && (!kSwap || mbar_wait(full(s), ph, ctx, 25)));
+                ok = __all_sync(0xffffffffu, mbar_wait(acc_full(b), bph, ctx, 24) && (!kRingScales || mbar_wait(full(s), ph, ctx, 25)));
                 if (!ok) break;
                 tcgen05_fence_after();
-                const uint32_t sc = base + L.scales + s * (C::kScales * 4);
+                const uint32_t sc = base + (kOwn ? L.own_scales + (kb - k0) * (kCols * 4) : L.scales + s * (C::kScales * 4));
                 const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + b * C::kBufCols + half * C::kPer;
                 auto given_back = [&]() {
                     tcgen05_fence_before();
                     __syncwarp();
                     if (lane == 0) {
                         mbar_arrive(acc_empty(b));
-                        if constexpr (kSwap) mbar_arrive(empty(s));
+                        if constexpr (kRingScales) mbar_arrive(empty(s));
                     }
                 };
                 if constexpr (kSwap) add_scaled_by_column(src, sc, sw_now, acc, given_back);
@@ -703,6 +757,7 @@ struct Fp8Problem {
     const uint8_t* w;
     int64_t ldw, k;
     bool dependent;                      // the kernel before is the quantizer of x
+    bool own;                            // x is dense: the product quantizes it
 };
 
 int encode_codes(EncodeTiledFn fn, CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int64_t ld, uint32_t box_rows) {
@@ -720,12 +775,12 @@ struct Fp8Choice {
 };
 // An arrangement's cost in microseconds: rounds of items times blocks of K in a run.  Per block: what the weights of one SM
 // take from HBM, or the tensor core and the epilogue; per item: filling and draining the pipeline, an exchange.
-template <int kCols, bool kSwap>
+template <int kCols, bool kSwap, bool kOwn>
 int consider(const Fp8Args& a, Fp8Choice& best) {
     static ActiveClusters active;
     int clusters[kMaxClusterLog + 1];
-    const auto kernel = fp8_gemm_kernel<kCols, kSwap>;
-    if (const int rc = active_clusters(active, reinterpret_cast<const void*>(kernel), Fp8Cfg<kCols, kSwap>::kThreads, kSmemMax, clusters))
+    const auto kernel = fp8_gemm_kernel<kCols, kSwap, kOwn>;
+    if (const int rc = active_clusters(active, reinterpret_cast<const void*>(kernel), Fp8Cfg<kCols, kSwap, kOwn>::kThreads, kSmemMax, clusters))
         return rc;
     const int64_t lanes = kSwap ? a.n : a.m, cols = kSwap ? a.m : a.n;
     const int64_t items = (lanes + 127) / 128 * ((cols + kCols - 1) / kCols);
@@ -776,38 +831,41 @@ int launch_fp8(Fp8Args a, const Fp8Problem& p, const Fp8Choice& c, int x_box, in
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return record_error_text("cuTensorMapEncodeTiled is not available");
     CUtensorMap map_x, map_w;
-    if (const int rc = encode_codes(fn, &map_x, p.x, a.m, p.k, p.ldx, (uint32_t)x_box)) return rc;
     if (const int rc = encode_codes(fn, &map_w, p.w, a.n, p.k, p.ldw, (uint32_t)w_box)) return rc;
+    if (p.own) map_x = map_w;                                           // not used
+    else if (const int rc = encode_codes(fn, &map_x, p.x, a.m, p.k, p.ldx, (uint32_t)x_box)) return rc;
     a.x_tiles = (a.m + x_tile - 1) / x_tile;
     const int64_t items = (int64_t)a.x_tiles * ((a.n + w_tile - 1) / w_tile);
     if (items > 0x3fffffff) return MIXFP4_E_SHAPE;
     a.items = (int)items;
     return launch_clusters(kernel, 1 << c.cluster_log, a.items < c.active ? a.items : c.active, threads, smem, p, map_x, map_w, a, st);
 }
-template <int kCols, bool kSwap>
+template <int kCols, bool kSwap, bool kOwn>
 int launch_single(Fp8Args a, const Fp8Problem& p, const Fp8Choice& c, cudaStream_t st) {
     a.cluster = 1 << c.cluster_log;
     a.stages = kMaxStages;
-    while (fp8_layout<kCols, kSwap>(a.stages, a.cluster).bytes > kSmemMax) --a.stages;
-    const auto kernel = fp8_gemm_kernel<kCols, kSwap>;
+    while (fp8_layout<kCols, kSwap, kOwn>(a.stages, a.cluster, a.blocks).bytes > kSmemMax) --a.stages;
+    const auto kernel = fp8_gemm_kernel<kCols, kSwap, kOwn>;
     constexpr int kX = kSwap ? kCols : 128, kW = kSwap ? 128 : kCols;
-    return launch_fp8(a, p, c, kX, kW, kX, kW, reinterpret_cast<const void*>(kernel), Fp8Cfg<kCols, kSwap>::kThreads,
-                      fp8_layout<kCols, kSwap>(a.stages, a.cluster).bytes, st);
+    return launch_fp8(a, p, c, kX, kW, kX, kW, reinterpret_cast<const void*>(kernel), Fp8Cfg<kCols, kSwap, kOwn>::kThreads,
+                      fp8_layout<kCols, kSwap, kOwn>(a.stages, a.cluster, a.blocks).bytes, st);
+}
+template <int kCols, bool kOwn>
+int few_rows(const Fp8Args& a, const Fp8Problem& p, cudaStream_t st) {
+    Fp8Choice best;
+    if (const int rc = consider<kCols, true, kOwn>(a, best)) return rc;
+    return best.cols ? launch_single<kCols, true, kOwn>(a, p, best, st) : MIXFP4_E_UNSUPPORTED;
 }
 
 int fp8_gemm(const Fp8Args& a, const Fp8Problem& p, cudaStream_t st) {
+    if (a.m <= 16) return p.own ? few_rows<16, true>(a, p, st) : few_rows<16, false>(a, p, st);
+    if (a.m <= 32) return p.own ? few_rows<32, true>(a, p, st) : few_rows<32, false>(a, p, st);
+    if (a.m <= 64) return p.own ? few_rows<64, true>(a, p, st) : few_rows<64, false>(a, p, st);
     Fp8Choice best;
-    int rc;
-    if (a.m <= 16) rc = consider<16, true>(a, best);
-    else if (a.m <= 32) rc = consider<32, true>(a, best);
-    else if (a.m <= 64) rc = consider<64, true>(a, best);
-    else if (!(rc = consider<128, false>(a, best))) rc = consider_pair(a, best);
-    if (rc) return rc;
+    if (const int rc = consider<128, false, false>(a, best)) return rc;
+    if (const int rc = consider_pair(a, best)) return rc;
     switch (best.cols) {
-        case 16: return launch_single<16, true>(a, p, best, st);
-        case 32: return launch_single<32, true>(a, p, best, st);
-        case 64: return launch_single<64, true>(a, p, best, st);
-        case 128: return launch_single<128, false>(a, p, best, st);
+        case 128: return launch_single<128, false, false>(a, p, best, st);
         case 256: return launch_fp8(a, p, best, 128, 128, 256, 256, reinterpret_cast<const void*>(fp8_pair_kernel), kPairThreads, kPairBytes, st);
         default: return MIXFP4_E_UNSUPPORTED;
     }
@@ -828,7 +886,7 @@ Fp8Args make_args(const float* sx, int64_t ldsx, const float* sw, int64_t m, int
                   int64_t ldy, int* status) {
     Fp8Args a = {};
     a.sx = sx; a.sw = sw; a.y = y; a.ldsx = ldsx; a.ldy = ldy;
-    a.m = (int)m; a.n = (int)n; a.blocks = (int)((k + kFp8Block - 1) / kFp8Block);
+    a.m = (int)m; a.n = (int)n; a.k = (int)k; a.blocks = (int)((k + kFp8Block - 1) / kFp8Block);
     a.out_dtype = out_dtype; a.status = status;
     a.y_vec = aligned(y, 32) && ldy * (out_dtype == MIXFP4_F32 ? 4 : 2) % 32 == 0;
     return a;
@@ -846,12 +904,12 @@ extern "C" int mixfp4_fp8_gemm(const uint8_t* x, int64_t ldx, const float* x_sca
     if (const int rc = check_product(w, ldw, w_scales, m, n, k, y, out_dtype, ldy)) return rc;
     if (ldx < k || lds < fp8_scale_rows(m)) return MIXFP4_E_SHAPE;
     if (!aligned(x, 16) || ldx % 16 != 0 || !aligned(x_scales, 16) || lds % 4 != 0) return MIXFP4_E_ALIGN;
-    return fp8_gemm(make_args(x_scales, lds, w_scales, m, n, k, y, out_dtype, ldy, status), Fp8Problem{x, ldx, w, ldw, k, false},
+    return fp8_gemm(make_args(x_scales, lds, w_scales, m, n, k, y, out_dtype, ldy, status), Fp8Problem{x, ldx, w, ldw, k, false, false},
                     static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int64_t mixfp4_fp8_workspace_bytes(int64_t m, int64_t k) {
-    if (m <= 0 || k <= 0) return 0;
+    if (m <= 0 || k <= 0 || fp8_quantizes_itself(m, k)) return 0;
     const int64_t kp = padded_k(k);
     return (m * kp + 15) / 16 * 16 + fp8_scale_rows(m) * (kp / kFp8Block) * 4;
 }
@@ -861,12 +919,22 @@ extern "C" int mixfp4_fp8_linear(const void* x, int dtype, int64_t m, int64_t ld
                                  void* workspace, int64_t workspace_bytes, int* status, void* stream) {
     if (!x) return MIXFP4_E_NULL;
     if (const int rc = check_product(w, ldw, w_scales, m, n, k, y, out_dtype, ldy)) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    Fp8Args a = make_args(nullptr, 0, w_scales, m, n, k, y, out_dtype, ldy, status);
+    if (fp8_quantizes_itself(m, k)) {
+        if (dtype != MIXFP4_BF16 && dtype != MIXFP4_F16 && dtype != MIXFP4_F32) return MIXFP4_E_DTYPE;
+        if (ldx < k) return MIXFP4_E_SHAPE;
+        a.x = x; a.ldx = ldx; a.x_dtype = dtype;
+        a.x_vec = aligned(x, 16) && ldx * (dtype == MIXFP4_F32 ? 4 : 2) % 16 == 0;
+        return fp8_gemm(a, Fp8Problem{nullptr, 0, w, ldw, k, false, true}, st);
+    }
     if (!workspace || workspace_bytes < mixfp4_fp8_workspace_bytes(m, k)) return MIXFP4_E_WORKSPACE;
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     const int64_t kp = padded_k(k), lds = fp8_scale_rows(m);
     float* scales = reinterpret_cast<float*>(codes + (m * kp + 15) / 16 * 16);
     if (const int rc = fp8_check_rows(x, dtype, m, k, ldx, codes, kp, scales, lds)) return rc;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (const int rc = fp8_quantize_rows(x, dtype, m, k, ldx, codes, kp, scales, lds, st)) return rc;
-    return fp8_gemm(make_args(scales, lds, w_scales, m, n, k, y, out_dtype, ldy, status), Fp8Problem{codes, kp, w, ldw, k, true}, st);
+    a.sx = scales;
+    a.ldsx = lds;
+    return fp8_gemm(a, Fp8Problem{codes, kp, w, ldw, k, true, false}, st);
 }

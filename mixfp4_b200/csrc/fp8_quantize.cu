@@ -13,72 +13,6 @@
 namespace mixfp4 {
 namespace {
 
-constexpr float kLargest = 448.0f;
-constexpr int kLaneElems = 16, kLanesPerRow = kFp8Block / kLaneElems;       // a lane holds 16 elements of a row's block
-
-// The larger magnitude, NaN if either is one (fmaxf would drop it).
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
-// 16 consecutive elements of a row from column c, zero past k.
-template <typename T>
-__device__ __forceinline__ void load16(const T* row, int64_t c, int64_t k, bool vec, float (&v)[kLaneElems]) {
-    if (vec && c + kLaneElems <= k) {
-        constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < kLaneElems / kPer; ++i) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
-            const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) v[i * kPer + j] = Elem<T>::load(e + j);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < kLaneElems; ++j) v[j] = c + j < k ? Elem<T>::load(row + c + j) : 0.0f;
-    }
-}
-
-__device__ __forceinline__ float largest_of(const float (&v)[kLaneElems]) {
-    float a = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kLaneElems; ++j) a = max_nan(a, fabsf(v[j]));
-    return a;
-}
-
-__device__ __forceinline__ float block_scale(float largest) {
-    const float s = __fdiv_rn(largest, kLargest);
-    return s == 0.0f ? 1.0f : s;
-}
-
-// x / s rounded once, for the 16 values of a lane.  One reciprocal for all of them and a residual step each:
-// q = x r, then q + (x - q s) r, which is the rounded quotient when r is the rounded reciprocal and nothing
-// underflows (Markstein 1990, theorem on final rounding).  Scales outside 2^+-100 take the division itself.
-__device__ __forceinline__ uint4 encode16(const float (&v)[kLaneElems], float s) {
-    float q[kLaneElems];
-    if (s > 0x1p-100f && s < 0x1p100f) {
-        const float r = __frcp_rn(s);
-#pragma unroll
-        for (int j = 0; j < kLaneElems; ++j) {
-            const float q0 = __fmul_rn(v[j], r);
-            q[j] = __fmaf_rn(__fmaf_rn(-q0, s, v[j]), r, q0);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < kLaneElems; ++j) q[j] = __fdiv_rn(v[j], s);
-    }
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[4 * i], q[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[4 * i + 2], q[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
-        w[i] = lo | (hi << 16);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // A group of eight lanes per row and block.  scales: [block][lds], a row's scales a column of it, so that the product reads
 // the scales of neighbouring rows together.
 template <typename T>
@@ -94,45 +28,49 @@ __global__ void __launch_bounds__(256) fp8_rows_kernel(const T* x, int64_t m, in
         if (!__any_sync(0xffffffffu, in)) break;
         const int64_t row = in ? i / blocks : 0, b = in ? i - row * blocks : 0;
         const int64_t c = b * kFp8Block + sub * kLaneElems;
-        float v[kLaneElems];
+        Raw<T> v;
         load16(x + row * ldx, c, in ? k : 0, vec, v);
-        float a = largest_of(v);
+        uint32_t a = largest_of(v);
 #pragma unroll
-        for (int d = 1; d < kLanesPerRow; d *= 2) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, d));
+        for (int d = 1; d < kLanesPerRow; d *= 2) a = larger<T>(a, __shfl_xor_sync(0xffffffffu, a, d));
         if (in) {
-            const float s = block_scale(a);
+            const float s = block_scale(magnitude<T>(a));
             *reinterpret_cast<uint4*>(codes + row * ldq + c) = encode16(v, s);
             if (sub == 0) scales[b * lds + row] = s;
         }
     }
 }
 
-// A CTA of 512 threads per 128 x 128 tile: 64 rows a pass, two passes, 32 elements a thread.
-constexpr int kTileThreads = 512, kTilePasses = 128 * kLanesPerRow / kTileThreads;
+// A CTA of 256 threads per 128 x 128 tile: 32 rows a pass, four passes, 64 elements a thread, kept as they were read: in 16 bits
+// four CTAs fit an SM, and the loads of one hide behind the arithmetic of the others (14336 x 4096 bf16: 33 us, 5.3 TB/s;
+// elements kept in fp32 by 512 threads, two CTAs an SM, 49 us; 512 threads and three CTAs 38 us; five CTAs of 256, 39 us).
+constexpr int kTileThreads = 256, kTilePasses = 128 * kLanesPerRow / kTileThreads;
 template <typename T>
-__global__ void __launch_bounds__(kTileThreads) fp8_tiles_kernel(const T* w, int64_t n, int64_t k, int64_t ldw, bool vec,
-                                                                 uint8_t* codes, int64_t ldq, float* scales) {
-    __shared__ float warp_max[kTileThreads / 32];
+__global__ void __launch_bounds__(kTileThreads, sizeof(T) == 2 ? 4 : 2) fp8_tiles_kernel(const T* w, int64_t n, int64_t k, int64_t ldw,
+                                                                                        bool vec, uint8_t* codes, int64_t ldq,
+                                                                                        float* scales) {
+    __shared__ uint32_t warp_max[kTileThreads / 32];
     const int64_t blocks = (k + kFp8Block - 1) / kFp8Block;
     const int64_t tile = blockIdx.x / blocks, b = blockIdx.x - tile * blocks;
     const int sub = threadIdx.x % kLanesPerRow, first = threadIdx.x / kLanesPerRow;
     const int64_t c = b * kFp8Block + sub * kLaneElems;
-    float v[kTilePasses][kLaneElems];
-    float a = 0.0f;
+    Raw<T> v[kTilePasses];
+    uint32_t a = 0;
 #pragma unroll
     for (int p = 0; p < kTilePasses; ++p) {
         const int64_t row = tile * kFp8Block + first + p * (kTileThreads / kLanesPerRow);
         load16(w + (row < n ? row : 0) * ldw, c, row < n ? k : 0, vec, v[p]);
-        a = max_nan(a, largest_of(v[p]));
     }
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, d));
+    for (int p = 0; p < kTilePasses; ++p) a = larger<T>(a, largest_of(v[p]));
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) a = larger<T>(a, __shfl_xor_sync(0xffffffffu, a, d));
     if (threadIdx.x % 32 == 0) warp_max[threadIdx.x / 32] = a;
     __syncthreads();
-    a = warp_max[0];
+    a = warp_max[threadIdx.x % (kTileThreads / 32)];
 #pragma unroll
-    for (int i = 1; i < kTileThreads / 32; ++i) a = max_nan(a, warp_max[i]);
-    const float s = block_scale(a);
+    for (int d = 1; d < kTileThreads / 32; d *= 2) a = larger<T>(a, __shfl_xor_sync(0xffffffffu, a, d));
+    const float s = block_scale(magnitude<T>(a));
     if (threadIdx.x == 0) scales[tile * blocks + b] = s;
 #pragma unroll
     for (int p = 0; p < kTilePasses; ++p) {

@@ -20,7 +20,6 @@ from . import _native as nat
 from .linear import _status_word
 
 FP8_BLOCK = 128
-_OUT_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _blocks(size: int) -> int:
@@ -119,6 +118,8 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     if x.ndim == 0 or x.shape[-1] == 0:
         raise ValueError(f"{what} must have at least one column")
     x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+    if x2.stride(0) >= x2.shape[1] and x2.stride(1) == 1:
+        return x2
     if x2.stride(1) != 1 or x2.stride(0) < x2.shape[1]:
         x2 = x2.reshape(1, -1) if x2.shape[0] == 1 and x2.stride(1) == 1 else x2.contiguous()
         if x2.stride(0) < x2.shape[1]:                   # a single row, whose stride can be any number
@@ -126,7 +127,6 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     return x2
 
 
-@torch.no_grad()
 def quantize_fp8_weight(w: torch.Tensor) -> FP8Weight:
     """A dense [n, k] weight (bf16, f16 or fp32, on the GPU) to codes and a scale for every 128 x 128 tile, in one pass."""
     if w.ndim != 2 or 0 in w.shape:
@@ -142,7 +142,6 @@ def quantize_fp8_weight(w: torch.Tensor) -> FP8Weight:
     return FP8Weight(codes[:, :k], scales)
 
 
-@torch.no_grad()
 def quantize_fp8_activations(x: torch.Tensor) -> FP8Activations:
     """Rows [..., K] to codes and a scale for every row and 128 columns: once for all the weights that read them."""
     x2 = _rows(x.detach(), "x")
@@ -158,7 +157,6 @@ def quantize_fp8_activations(x: torch.Tensor) -> FP8Activations:
     return FP8Activations(codes[:, :k], scales, x.shape, x.dtype)
 
 
-@torch.no_grad()
 def dequantize_fp8(q: FP8Weight | FP8Activations, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """code * scale as a dense matrix, rounded once."""
     if dtype not in nat.DTYPE_CODE:
@@ -175,46 +173,45 @@ def dequantize_fp8(q: FP8Weight | FP8Activations, dtype: torch.dtype = torch.bfl
     return out
 
 
-@torch.no_grad()
 def fp8_linear(x: torch.Tensor | FP8Activations, weight: FP8Weight, *, bias: torch.Tensor | None = None,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y = x @ W^T (+ bias) on block-scaled FP8 operands.  x: a dense tensor [..., K] (bf16, f16 or fp32), quantized within
     the call, or what `quantize_fp8_activations` made of one.  out_dtype: bf16, f16 or fp32 (default: x's dtype).  A product
     whose device-side waits run out reports through `gemm_status()`, like the other GEMMs."""
-    k, n, device = weight.k, weight.n, weight.device
-    quantized = isinstance(x, FP8Activations)
+    codes, n, k = weight.codes, weight.n, weight.k
+    device, shape = codes.device, x.shape
     out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in _OUT_DTYPES:
+    out_code = nat.DTYPE_CODE.get(out_dtype)
+    if out_code is None:
         raise TypeError("out_dtype must be bfloat16, float16 or float32")
-    if x.shape[-1] != k:
-        raise ValueError(f"x has K={x.shape[-1]}, the weight K={k}")
+    if shape[-1] != k:
+        raise ValueError(f"x has K={shape[-1]}, the weight K={k}")
     if x.device != device:
         raise ValueError(f"x is on {x.device}, the weight on {device}")
-    nat.require_cuda(weight.codes, "the weight")
-    lead = x.shape[:-1]
+    nat.require_cuda(codes, "the weight")
+    quantized = isinstance(x, FP8Activations)
     x2 = x.codes if quantized else _rows(x, "x")
     m = x2.shape[0]
     y = torch.empty((m, n), dtype=out_dtype, device=device)
     if m:
         lib = nat.lib()
-        w = weight.codes.data_ptr(), weight.codes.stride(0), weight.scales.data_ptr()
         with nat.on_device(device):
             stream = nat.stream_ptr(device)
             if quantized:
-                st = lib.mixfp4_fp8_gemm(x2.data_ptr(), x2.stride(0), x.scales.data_ptr(), x.scales.stride(1), *w,
-                                         m, n, k, y.data_ptr(), nat.DTYPE_CODE[out_dtype], n, _status_word(device).data_ptr(),
-                                         stream)
+                st = lib.mixfp4_fp8_gemm(x2.data_ptr(), x2.stride(0), x.scales.data_ptr(), x.scales.stride(1), codes.data_ptr(),
+                                         codes.stride(0), weight.scales.data_ptr(), m, n, k, y.data_ptr(), out_code, n,
+                                         _status_word(device).data_ptr(), stream)
                 nat.check("mixfp4_fp8_gemm", st)
             else:
                 nbytes = lib.mixfp4_fp8_workspace_bytes(m, k)
-                work = torch.empty(nbytes, dtype=torch.uint8, device=device)      # a captured graph's own
-                st = lib.mixfp4_fp8_linear(x2.data_ptr(), nat.DTYPE_CODE[x2.dtype], m, x2.stride(0), *w, n, k,
-                                           y.data_ptr(), nat.DTYPE_CODE[out_dtype], n, work.data_ptr(), nbytes,
-                                           _status_word(device).data_ptr(), stream)
+                work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None      # a captured graph's own
+                st = lib.mixfp4_fp8_linear(x2.data_ptr(), nat.DTYPE_CODE[x2.dtype], m, x2.stride(0), codes.data_ptr(),
+                                           codes.stride(0), weight.scales.data_ptr(), n, k, y.data_ptr(), out_code, n,
+                                           nat.ptr(work), nbytes, _status_word(device).data_ptr(), stream)
                 nat.check("mixfp4_fp8_linear", st)
     if bias is not None:
         y += bias.to(y.dtype)
-    return y if len(lead) == 1 else y.reshape(*lead, n)
+    return y if len(shape) == 2 else y.reshape(*shape[:-1], n)
 
 
 class FP8Linear(nn.Module):

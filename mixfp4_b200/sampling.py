@@ -17,6 +17,9 @@ from . import _native as nat
 
 def _setting(value, name: str, dtype: torch.dtype, rows: int, device, low: float, high: float):
     """(tensor or None, number): a checked number for all rows, or a tensor with one for each."""
+    kind = type(value)
+    if (kind is float and dtype is torch.float32 or kind is int) and low <= value <= high:
+        return None, value
     if isinstance(value, torch.Tensor):
         if value.dtype != dtype:
             raise TypeError(f"{name} must be a number or a {dtype} tensor")
@@ -32,7 +35,6 @@ def _setting(value, name: str, dtype: torch.dtype, rows: int, device, low: float
     return None, value
 
 
-@torch.no_grad()
 def sample_logits(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
                   return_logprob: bool = False) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """Tokens int64 [...] for logits [..., V] (bf16, f16 or fp32) and random numbers `uniform` fp32 [...] in [0, 1).
