@@ -5,7 +5,7 @@
 //   token   the first index, in the vocabulary's order, at which the kept weights add up to more than u times their sum
 //
 // Nothing is sorted.  A cluster of CTAs holds a row in shared memory (one HBM read) and narrows the cut down by
-// histograms: 1024 bins of equal width over the logits that have a weight at all, then 1024 bins of the keys (a monotone
+// histograms: 512 bins of equal width over the logits that have a weight at all, then 512 bins of the keys (a monotone
 // integer of the value) in the bin that the cut falls in, until that bin is one value; equal values are counted off by
 // index.  Every CTA adds the cluster's histograms up for itself: one cluster barrier a step, none to hand a result round.
 // Where the first histogram leaves at most 256 candidates for a top-k (the usual settings), one CTA takes them all and
@@ -28,7 +28,7 @@
 namespace mixfp4 {
 namespace {
 
-constexpr int kSampleThreads = 1024, kSampleWarps = kSampleThreads / 32, kBins = 1024;
+constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32, kBinsLog = 9, kBins = 1 << kBinsLog;
 static_assert(kBins == kSampleThreads, "a thread owns a bin");
 constexpr int kMaxRanks = 8;
 constexpr int64_t kMaxSlice = 65536, kMaxVocab = kMaxRanks * kMaxSlice - 128;
@@ -78,7 +78,7 @@ struct Row {
 // What the CTAs of a cluster tell one another; two sets in turn, so that a set is written again only after a barrier that
 // every reader of it has passed.
 struct Slots {
-    float largest[kMaxRanks];
+    float largest[kMaxRanks], least_of_groups[kMaxRanks];
     uint32_t count[kMaxRanks];
     u64 mass[kMaxRanks];
 };
@@ -91,7 +91,7 @@ struct Shared {
     Slots slots[2];
     u64 warp_mass[kSampleWarps];
     uint32_t warp_count[kSampleWarps];
-    float warp_max[kSampleWarps];
+    float warp_max[kSampleWarps], warp_least[kSampleWarps];
     u64 found_before;
     uint32_t found_bin, found_size, few_count;
 };
@@ -124,6 +124,7 @@ __device__ __forceinline__ uint32_t add_rank32(uint32_t addr, uint32_t v) {
     return was;
 }
 __device__ __forceinline__ void meet(int ranks) {        // all threads of the cluster; writes before are seen after
+    __syncwarp();
     if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     else __syncthreads();
 }
@@ -279,7 +280,7 @@ struct Sampler {
         if (lane == 31) s.warp_mass[warp] = up;
         if (threadIdx.x == 0) s.found_bin = kBins;
         __syncthreads();
-        u64 ahead = add_up(s.warp_mass[lane]);           // the warps' sums, added up by every warp
+        u64 ahead = add_up(lane < kSampleWarps ? s.warp_mass[lane] : 0);      // the warps' sums, added up by every warp
         if (goal == 0) goal = share_of(p, before + __shfl_sync(0xffffffffu, ahead, 31) - out);
         ahead = __shfl_sync(0xffffffffu, ahead, warp > 0 ? warp - 1 : 0);
         const u64 hi = before + (warp > 0 ? ahead : 0) + up, lo = hi - own;
@@ -310,7 +311,7 @@ struct Sampler {
         for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
         if (lane == 0) s.warp_mass[warp] = v;
         __syncthreads();
-        u64 all = s.warp_mass[lane];
+        u64 all = lane < kSampleWarps ? s.warp_mass[lane] : 0;
 #pragma unroll
         for (int d = 16; d > 0; d /= 2) all += __shfl_xor_sync(0xffffffffu, all, d);
         __syncthreads();
@@ -325,7 +326,7 @@ struct Sampler {
         if (a.logprob) a.logprob[r] = greedy ? 0.0f : (float)((x == largest ? 0.0 : ((double)x - top) * inv_t) - log_of(total));
     }
 
-    // At most kFew candidates, the elements of the linear bins up to `bin`: rank 0 takes them all, four threads to each, and
+    // At most kFew candidates, the elements of the linear bins up to `bin`: rank 0 takes them all, two threads to each, and
     // adds up what goes before it, by value and then, of the kept ones, by index.
     __device__ void choose_from_few(int64_t r, uint32_t bin, uint32_t k, double p, u64 lowest, double u) {
         const uint32_t count_at = of_rank(shared_addr(&s.few_count), 0), few_at = of_rank(shared_addr(s.few), 0);
@@ -340,27 +341,29 @@ struct Sampler {
                 if (at < kFew) st_rank64(few_at + at * 8, (u64)Row<T>::key(x[j]) << 32 | (uint32_t)~index);
             }
         }
+        constexpr uint32_t kParts = kSampleThreads / kFew;
         meet(a.ranks);
         if (rank != 0) return;
-        const uint32_t n = min(s.few_count, kFew), i = threadIdx.x / 4, part = threadIdx.x % 4;
+        const uint32_t n = min(s.few_count, kFew), i = threadIdx.x / kParts, part = threadIdx.x % kParts;
         if (threadIdx.x < n) s.few_weight[threadIdx.x] = weight(value_of((uint32_t)(s.few[threadIdx.x] >> 32)));
         __syncthreads();
         const u64 order = i < n ? s.few[i] : 0, w = i < n ? s.few_weight[i] : 0;
         const float x = value_of((uint32_t)(order >> 32));
-        auto four = [](u64 v) {
-            v += __shfl_xor_sync(0xffffffffu, v, 1);
-            return v + __shfl_xor_sync(0xffffffffu, v, 2);
+        auto join = [](u64 v) {
+#pragma unroll
+            for (int d = 1; d < (int)kParts; d *= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+            return v;
         };
         u64 mass = 0;
         uint32_t ahead = 0;
 #pragma unroll 2
-        for (uint32_t j = part; j < n; j += 4) {
+        for (uint32_t j = part; j < n; j += kParts) {
             const bool before = s.few[j] > order;
             mass += before ? s.few_weight[j] : 0;
             ahead += before;
         }
-        mass = four(mass);
-        ahead = (uint32_t)four(ahead);
+        mass = join(mass);
+        ahead = (uint32_t)join(ahead);
         bool kept = i < n && ahead < k;
         const u64 of_k = block_sum(kept && part == 0 ? w : 0);
         kept = kept && (p >= 1.0 || mass < share_of(p, of_k)) && w >= lowest;
@@ -368,8 +371,8 @@ struct Sampler {
         const u64 total = block_sum(kept && part == 0 ? w : 0), goal = target_of(u, total);
         u64 at = 0;
 #pragma unroll 2
-        for (uint32_t j = part; j < n; j += 4) at += (uint32_t)s.few[j] > (uint32_t)order ? s.few_weight[j] : 0;      // a lower index
-        at = four(at);
+        for (uint32_t j = part; j < n; j += kParts) at += (uint32_t)s.few[j] > (uint32_t)order ? s.few_weight[j] : 0;      // a lower index
+        at = join(at);
         if (part == 0 && kept && goal >= at && goal < at + w) answer(r, (int)~(uint32_t)order, x, false, total);
     }
 
@@ -406,20 +409,43 @@ struct Sampler {
                 for (int j = 0; j < kPer; ++j) most = fmaxf(most, Elem<T>::load(reinterpret_cast<const T*>(&v[i]) + j));
             }
         }
+        // The largest; and the least of the maxima of so many groups of lanes that there are k of them at least: no fewer than
+        // k elements reach it, so a top-k need not look below.
+        const int groups = kSampleWarps * ranks;
+        float least = k <= groups * 32 ? most : kNegInf;
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        if (lane == 0) s.warp_max[warp] = most;
+        for (int d = 1; d < 32; d *= 2) {
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            if (groups * (16 / d) >= k) least = most;
+        }
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, d));
+        if (lane == 0) {
+            s.warp_max[warp] = most;
+            s.warp_least[warp] = least;
+        }
         __syncthreads();
         if (warp == 0) {
-            most = s.warp_max[lane];
+            most = s.warp_max[lane % kSampleWarps];
+            least = s.warp_least[lane % kSampleWarps];
 #pragma unroll
-            for (int d = 16; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            if (lane < ranks) st_rank32(of_rank(shared_addr(&s.slots[0].largest[rank]), lane), __float_as_uint(most));
+            for (int d = 16; d > 0; d /= 2) {
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                least = fminf(least, __shfl_xor_sync(0xffffffffu, least, d));
+            }
+            if (lane < ranks) {
+                st_rank32(of_rank(shared_addr(&s.slots[0].largest[rank]), lane), __float_as_uint(most));
+                st_rank32(of_rank(shared_addr(&s.slots[0].least_of_groups[rank]), lane), __float_as_uint(least));
+            }
         }
         meet(ranks);
         largest = kNegInf;
+        float reached_by_k = -kNegInf;
 #pragma unroll 1
-        for (int q = 0; q < ranks; ++q) largest = fmaxf(largest, s.slots[0].largest[q]);
+        for (int q = 0; q < ranks; ++q) {
+            largest = fmaxf(largest, s.slots[0].largest[q]);
+            reached_by_k = fminf(reached_by_k, s.slots[0].least_of_groups[q]);
+        }
         top = (double)fminf(largest, FLT_MAX);
         if (largest == kNegInf) {                        // nothing to choose from
             if (rank == 0 && threadIdx.x == 0) {
@@ -441,12 +467,13 @@ struct Sampler {
             const bool by_mass = stage == 1;
             // the mass of the equal values that the cut by count leaves out
             const u64 out = by_mass && cut.equal > cut.ties ? (u64)(cut.equal - cut.ties) * weight(cut.value) : 0;
+            const float from = by_mass ? cut.value : fmaxf(cut.value, reached_by_k);
             u64 goal = by_mass ? 0 : (u64)k, before = 0;
             uint32_t bin = 0, lo = 0, hi = 0;
 #pragma unroll 1
-            for (int level = 0; level < 5; ++level) {    // 32 bits of a key, 10 a level
+            for (int level = 0; level < 5; ++level) {    // 32 bits of a key, 9 a level
                 const uint32_t span = hi - lo;
-                const int shift = span < (uint32_t)kBins ? 0 : 22 - __clz(span);
+                const int shift = span < (uint32_t)kBins ? 0 : 32 - kBinsLog - __clz(span);
 #pragma unroll 1
                 for (int c = c0 + lane; c < c1; c += 32) {
                     float x[4];
@@ -456,7 +483,7 @@ struct Sampler {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         at[j] = linear(x[j]);
-                        hit[j] = x[j] >= cut.value && (level == 0 || at[j] == bin);
+                        hit[j] = x[j] >= from && (level == 0 || at[j] == bin);
                     }
                     if (!(hit[0] || hit[1] || hit[2] || hit[3])) continue;
                     if (level > 0) {
@@ -518,7 +545,7 @@ struct Sampler {
             ties_here = __reduce_add_sync(0xffffffffu, ties_here);
             if (lane == 0) s.warp_count[warp] = ties_here;
             __syncthreads();
-            const uint32_t up = (uint32_t)add_up(s.warp_count[lane]);
+            const uint32_t up = (uint32_t)add_up(lane < kSampleWarps ? s.warp_count[lane] : 0);
             if (warp == 0) {
                 const uint32_t all = __shfl_sync(0xffffffffu, up, 31);
                 if (lane < ranks) st_rank32(of_rank(shared_addr(&s.slots[1].count[rank]), lane), all);
@@ -593,7 +620,7 @@ struct Sampler {
             for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             if (lane == 0) s.warp_mass[warp] = sum;
             __syncthreads();
-            const u64 up = add_up(s.warp_mass[lane]);
+            const u64 up = add_up(lane < kSampleWarps ? s.warp_mass[lane] : 0);
             if (warp == 0) {
                 const u64 all = __shfl_sync(0xffffffffu, up, 31);
                 if (lane < ranks) st_rank64(of_rank(shared_addr(&s.slots[0].mass[rank]), lane), all);
@@ -613,7 +640,7 @@ struct Sampler {
 };
 
 template <typename T, bool kResident>
-__global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleArgs a) {
     __shared__ __align__(16) Shared s;
     extern __shared__ __align__(16) uint8_t sample_smem[];
     const int64_t r = blockIdx.x / a.ranks;
@@ -656,7 +683,7 @@ int sample(SampleArgs& a, int64_t rows, cudaStream_t st) {
     auto slice = [&](int ranks) { return ((int64_t)a.vocab + 2 * kPer - 2) / kPer / ranks + 1; };      // granules of a CTA, at most
     // as many CTAs to a row as keep the SMs busy, a thousand elements each at least; more where the slice would be too long
     int ranks = 1;
-    while (ranks < kMaxRanks && rows * ranks * 2 <= 148 && a.vocab / (ranks * 2) >= 1024) ranks *= 2;
+    while (ranks < kMaxRanks && rows * ranks * 2 <= 296 && a.vocab / (ranks * 2) >= 1024) ranks *= 2;
     while (ranks < kMaxRanks && (slice(ranks) * 16 > (int64_t)kSampleSmem || slice(ranks) * kPer > kMaxSlice)) ranks *= 2;
     a.ranks = ranks;
     const size_t smem = (size_t)slice(ranks) * 16;
