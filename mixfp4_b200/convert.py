@@ -14,7 +14,8 @@ Checkpoint format (`torch.save` of plain tensors and python scalars, no code obj
         "global_scale": f32 [1], "n": int, "k": int, "rotation": str | None, "mode": str,
         "activation_mode": str | None, "bias": tensor | None}}}
 The bytes are the canonical layout of include/mixfp4_b200.h (the one the parity tests hash);
-the kernel layout and the decode tables are rebuilt at load time.
+the kernel layout and the decode tables are rebuilt at load time.  A layer in block-scaled FP8 has instead
+    {"mode": "fp8", "codes": u8 [n, k] (E4M3), "scales": f32 [ceil(n/128), ceil(k/128)], "n": int, "k": int, "bias": tensor | None}
 """
 
 from __future__ import annotations
@@ -25,6 +26,7 @@ from typing import Any, Iterator
 import torch
 from torch import nn
 
+from .fp8 import FP8Linear, FP8Weight
 from .linear import MixFP4Linear
 from .quant import PackedWeight
 
@@ -61,7 +63,8 @@ def _set_submodule(model: nn.Module, name: str, new: nn.Module) -> None:
 @torch.no_grad()
 def quantize_model_weights(model: nn.Module, weight_mode: str = "oracle16", *, rotation: str = "identity",
                            per_module_rotation: dict[str, str] | None = None, device=None,
-                           activation_mode: str | None = None) -> list[dict[str, Any]]:
+                           activation_mode: str | None = None,
+                           per_module_mode: dict[str, str] | None = None) -> list[dict[str, Any]]:
     """Replace every linear of ``model`` (heads excluded) by a packed MixFP4Linear, in place.
 
     weight_mode: a format region of `quant_mixfp4_granularity` ("oracle16", "n8k64", ...);
@@ -71,23 +74,43 @@ def quantize_model_weights(model: nn.Module, weight_mode: str = "oracle16", *, r
     activation_mode: format region of the activation fake-quantization each converted layer
     applies to its (rotated) input, as the reference's ActivationHooks do (modeling.py:640-705);
     None / "bf16" leaves the activations in bf16.
+    per_module_mode: module name -> weight mode of its own.  "fp8" (as a weight_mode too) makes it an `FP8Linear`, block-scaled
+    FP8 weight and activations without a rotation, for layers that four bits hurt; output heads, which the walk leaves out,
+    are converted when they are named here.
     Returns one row per converted layer (name, type, layer index, shape, share of E0M3 blocks,
     packed bytes)."""
-    if weight_mode in {"high_precision", "fp16", "bf16"}:
-        return []
+    own_mode = per_module_mode or {}
+    linears = dict(named_linears(model))
+    modules = dict(model.named_modules())
+    for name in own_mode:
+        if not isinstance(modules.get(name), nn.Linear):
+            raise KeyError(f"per_module_mode names {name!r}, which is not a linear of the model")
+        linears.setdefault(name, modules[name])
     rows = []
-    for name, linear in list(named_linears(model)):
+    for name, linear in linears.items():
+        mode = own_mode.get(name, weight_mode)
+        if mode in {"high_precision", "fp16", "bf16"}:
+            continue
+        if mode == "fp8":
+            layer = FP8Linear.from_linear(linear, device=device)
+            _set_submodule(model, name, layer)
+            rows.append({
+                "module_name": name, "module_type": module_type(name), "layer_idx": layer_index(name),
+                "out_features": layer.out_features, "in_features": layer.in_features, "transform": "identity",
+                "format_granularity": mode, "e0_ratio": None, "packed_bytes": layer.weight_fp8.nbytes(),
+            })
+            continue
         chosen = per_module_rotation.get(name, rotation) if per_module_rotation else rotation
         chosen = None if chosen in (None, "identity") else chosen
-        layer = MixFP4Linear.from_linear(linear, rotation=chosen, mode=weight_mode, device=device,
+        layer = MixFP4Linear.from_linear(linear, rotation=chosen, mode=mode, device=device,
                                          activation_mode=activation_mode)
-        layer.weight_mode = weight_mode
+        layer.weight_mode = mode
         _set_submodule(model, name, layer)
         packed = layer.packed
         rows.append({
             "module_name": name, "module_type": module_type(name), "layer_idx": layer_index(name),
             "out_features": layer.out_features, "in_features": layer.in_features, "transform": chosen or "identity",
-            "format_granularity": weight_mode,
+            "format_granularity": mode,
             "e0_ratio": float(packed.format_ids().float().mean().item()),
             "packed_bytes": packed.nbytes(),
         })
@@ -95,7 +118,7 @@ def quantize_model_weights(model: nn.Module, weight_mode: str = "oracle16", *, r
 
 
 def packed_state(model: nn.Module) -> dict[str, Any]:
-    """The checkpoint dictionary of every MixFP4Linear in ``model`` (canonical bytes, on the CPU)."""
+    """The checkpoint dictionary of every MixFP4Linear and FP8Linear in ``model`` (canonical bytes, on the CPU)."""
     layers = {}
     for name, module in model.named_modules():
         if isinstance(module, MixFP4Linear):
@@ -105,6 +128,12 @@ def packed_state(model: nn.Module) -> dict[str, Any]:
                 "global_scale": p.global_scale.cpu(), "n": p.n, "k": p.k, "rotation": p.rotation,
                 "mode": getattr(module, "weight_mode", "oracle16"),
                 "activation_mode": module.activation_mode,
+                "bias": None if module.bias is None else module.bias.detach().cpu(),
+            }
+        elif isinstance(module, FP8Linear):
+            layers[name] = {
+                "mode": "fp8", "codes": module.codes.contiguous().view(torch.uint8).cpu(), "scales": module.scales.cpu(),
+                "n": module.out_features, "k": module.in_features,
                 "bias": None if module.bias is None else module.bias.detach().cpu(),
             }
     return {"format": FORMAT_NAME, "version": FORMAT_VERSION, "layers": layers}
@@ -135,9 +164,14 @@ def load_packed(model: nn.Module, path_or_state, *, device=None, strict: bool = 
         shape = (old.out_features, old.in_features) if hasattr(old, "out_features") else None
         if strict and shape is not None and shape != (entry["n"], entry["k"]):
             raise ValueError(f"{name}: checkpoint holds {entry['n']}x{entry['k']}, the model {shape[0]}x{shape[1]}")
+        bias = None if entry["bias"] is None else entry["bias"].to(device)
+        if entry.get("mode") == "fp8":
+            weight = FP8Weight.from_tensors(entry["codes"].to(device), entry["scales"].to(device))
+            _set_submodule(model, name, FP8Linear(weight, bias))
+            done.append(name)
+            continue
         packed = PackedWeight(entry["codes"].to(device), entry["scales"].to(device), entry["fmt"].to(device),
                               entry["global_scale"].to(device), entry["n"], entry["k"], entry["rotation"])
-        bias = None if entry["bias"] is None else entry["bias"].to(device)
         layer = MixFP4Linear(packed, bias, entry.get("activation_mode"))
         layer.weight_mode = entry.get("mode", "oracle16")
         _set_submodule(model, name, layer)

@@ -17,9 +17,12 @@
 // words only, so a bin's sum is two words, and whoever overflows the low one adds the carry to the high one: one addition
 // for all but the largest few thousandths of the weights.
 //
-// What bounds it: a row of a small batch takes a dozen dependent steps (passes over shared memory, cluster barriers), and
-// code that runs once or twice: instruction fetch counts, so every pass has one copy (86 KB of unrolled passes took 70 us for
-// one row of 128256 logits with top-k and top-p, a third of that code 39 us).  Large batches: the fp64 operations of the weights.
+// What bounds it.  A row of a small batch takes a dozen dependent steps (passes over shared memory, cluster barriers), and code
+// that runs once or twice: instruction fetch counts, so every pass has one copy (unrolled passes, 86 KB of code, took 70 us for
+// one row of 128256 logits with top-k and top-p; this takes 13).  Large batches: the fp64 operations of the weights, in a pass
+// with all of them 14 us for the 64 K elements of an SM, and the histogram's additions in shared memory.
+// Measured and not kept: lists of a warp's few elements of interest, sorting the candidates, sums of what a top-p cannot reach
+// beside the histogram (each more code than it saved time: 64 mixed rows 61 us, so 69 to 79).
 
 #include <float.h>
 
@@ -40,11 +43,15 @@ constexpr float kNegInf = -__builtin_huge_valf();
 
 typedef unsigned long long u64;
 
+// Ordinary loads: what they read may have been written while this kernel was already running.
+template <typename T>
+__device__ __forceinline__ T ld_global(const T* p) { return *p; }
+
 template <typename T, typename All>
 struct Setting {                                         // a value for each row, or one for all
     const T* each;
     All all;
-    __device__ All of(int64_t row) const { return each ? (All)__ldg(each + row) : all; }
+    __device__ All of(int64_t row) const { return each ? (All)ld_global(each + row) : all; }
 };
 struct SampleArgs {
     const void* logits;
@@ -174,7 +181,7 @@ struct Sampler {
     // lies outside the row count as -inf (the larger of NaN and a number is the number).
     __device__ uint4 fetch(int g) const {
         const int i = g * kPer - skew;
-        uint4 u = i >= 0 && i + kPer <= a.vocab ? __ldg(reinterpret_cast<const uint4*>(row + i)) : fetch_end(row, i, a.vocab);
+        uint4 u = i >= 0 && i + kPer <= a.vocab ? ld_global(reinterpret_cast<const uint4*>(row + i)) : fetch_end(row, i, a.vocab);
         if constexpr (sizeof(T) == 4) {
             float* e = reinterpret_cast<float*>(&u);
 #pragma unroll
@@ -378,10 +385,6 @@ struct Sampler {
 
     __device__ void run(int64_t r) {
         const int ranks = a.ranks;
-        const double t = a.temperature.of(r), p = a.top_p.of(r), u = (double)__ldg(a.uniform + r);
-        const int k = a.top_k.of(r);
-        const bool greedy = !(t > 0.0);
-        const u64 lowest = greedy ? 0 : (u64)__double2ll_rn(fmin(fmax(a.min_p.of(r), 0.0), 1.0) * kOne);
         // the row's granules, the cluster's share, the warps' shares: contiguous, so that indices rise with rank, warp, lane
         const int granules = (a.vocab + skew + kPer - 1) / kPer, per_rank = (granules + ranks - 1) / ranks;
         first = min(rank * per_rank, granules);
@@ -394,6 +397,13 @@ struct Sampler {
         clear(1);
         if (threadIdx.x < kSteps) s.octave[threadIdx.x] = octave_step(threadIdx.x);
         if (threadIdx.x == 0) s.few_count = 0;
+        // Nothing of the caller's has been read so far: up to here the kernel runs under the tail of the one before.
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        const double t = a.temperature.of(r), p = a.top_p.of(r), u = (double)ld_global(a.uniform + r);
+        const int k = a.top_k.of(r);
+        const bool greedy = !(t > 0.0);
+        const u64 lowest = greedy ? 0 : (u64)__double2ll_rn(fmin(fmax(a.min_p.of(r), 0.0), 1.0) * kOne);
 
         float most = kNegInf;
         constexpr int kAhead = 4;                        // granules of a lane on their way at once
@@ -666,12 +676,16 @@ int launch_sample(const SampleArgs& a, int64_t rows, size_t smem, cudaStream_t s
     cfg.blockDim = dim3(kSampleThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)a.ranks;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    // One that starts under the tail of the kernel before gets the SMs in the order in which they fall free, two CTAs to each:
+    // only where every CTA would have an SM to itself anyway (64 rows of 128256, 256 CTAs: 61 us without, 67 us with it).
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = rows * a.ranks <= 148 ? 2 : 1;
     const auto kernel = sample_kernel<T, kResident>;
     MIXFP4_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, a));
     return check_launch("sample_kernel");

@@ -2,13 +2,15 @@
 mixed-FP4 layers, to report tokens/s and the share of a decode step spent in the mixed-FP4 GEMVs.
 
     python -m mixfp4_b200.llama_decode [--layers 32] [--batch 1] [--prompt 2048] [--tokens 32]
+                                       [--head fp8] [--temperature 0.8 --top-k 50 --top-p 0.95 --min-p 0.0]
     python -m torch.distributed.run --nproc-per-node 8 -m mixfp4_b200.llama_decode --tp 8 ...
 
 Architecture: hidden 4096, 32 query / 8 KV heads of 128, FFN 14336, RMSNorm, RoPE (theta 5e5),
 vocab 128256, bf16 KV cache.  Weights are seeded synthetic tensors (no checkpoint is available
 offline), quantized on the device layer by layer; the prompt is uniform random token ids.
 Everything that is not a linear -- norms, RoPE, attention over the KV cache, SiLU, the bf16
-embedding and output head -- runs as stock PyTorch operators: those are not part of the
+embedding and output head -- runs as stock PyTorch operators (--head fp8: the output head in block-scaled FP8;
+--temperature: a decode step ends with a token drawn by `sample_logits`): those are not part of the
 mixed-FP4 path, they are here so that the linears run in their real data flow (grouped q/k/v and
 gate/up launches, chained launches, batch rows = sequences).  The prompt is prefilled through the
 tcgen05 GEMM path, the decode steps are captured in one CUDA graph per step shape.
@@ -74,9 +76,13 @@ def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
 
 
 class Decoder:
-    def __init__(self, layers: int, batch: int, max_len: int, device, rank: int = 0, world: int = 1, weights=None):
+    def __init__(self, layers: int, batch: int, max_len: int, device, rank: int = 0, world: int = 1, weights=None,
+                 head: str = "bf16"):
         """weights: the `.weights` of another Decoder with the same layers and ranks, to share the
-        packed tensors between harness runs at different batch sizes."""
+        packed tensors between harness runs at different batch sizes.  head: "bf16", or "fp8" for an
+        output head in block-scaled FP8."""
+        if head not in ("bf16", "fp8"):
+            raise ValueError(f"unknown head={head!r}")
         self.device, self.batch, self.max_len, self.rank, self.world = device, batch, max_len, rank, world
         if HEADS % world or KV_HEADS % world:
             raise ValueError("the tensor-parallel degree must divide 8 KV heads")
@@ -90,6 +96,7 @@ class Decoder:
             weights = (stack, embed, head)
         self.weights = weights
         self.layers, self.embed, self.head = weights
+        self.head_fp8 = mx.quantize_fp8_weight(self.head) if head == "fp8" else None
         self.final_norm = torch.ones(HIDDEN, dtype=torch.bfloat16, device=device)
         self.k_cache = [torch.zeros((batch, self.kv_heads, max_len, HEAD_DIM), dtype=torch.bfloat16, device=device) for _ in self.layers]
         self.v_cache = [torch.zeros_like(c) for c in self.k_cache]
@@ -148,7 +155,7 @@ class Decoder:
             d = self.row_parallel(act, layer.down)
             h = d.view(b, t, HIDDEN) if self.linears_only else h2 + d.view(b, t, HIDDEN)
         last = rms_norm(h[:, -1], self.final_norm)
-        return last @ self.head.T
+        return last @ self.head.T if self.head_fp8 is None else mx.fp8_linear(last, self.head_fp8)
 
 
 def _time_graph(fn, steps: int) -> float:
@@ -175,13 +182,15 @@ def _time_graph(fn, steps: int) -> float:
 
 @torch.no_grad()
 def run(layers: int = 32, batch: int = 1, prompt: int = 2048, tokens: int = 32, device=None, tp: int = 1,
-        weights=None, keep: dict | None = None) -> dict:
+        weights=None, keep: dict | None = None, head: str = "bf16", sampling: dict | None = None) -> dict:
     """tp > 1: torch.distributed must be initialised with `tp` ranks (one per GPU); times are the
     maximum over ranks.  weights / keep: pass keep={} to receive the model's packed weights in
-    keep["weights"], and hand them back as `weights` to run another batch size without rebuilding."""
+    keep["weights"], and hand them back as `weights` to run another batch size without rebuilding.
+    head: see Decoder.  sampling: settings of `sample_logits` (temperature, top_k, top_p, min_p); the tokens are
+    then drawn, within the timed decode step, instead of the largest logit taken outside it."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     rank = dist.get_rank() if tp > 1 else 0
-    model = Decoder(layers, batch, prompt + tokens + 1, device, rank, tp, weights)
+    model = Decoder(layers, batch, prompt + tokens + 1, device, rank, tp, weights, head)
     if keep is not None:
         keep["weights"] = model.weights
     gen = torch.Generator(device=device).manual_seed(5)
@@ -197,9 +206,14 @@ def run(layers: int = 32, batch: int = 1, prompt: int = 2048, tokens: int = 32, 
     prefill_ms = e0.elapsed_time(e1)
     assert torch.isfinite(logits).all()
     # decode: one token per sequence at the position after the prompt, cache length prompt + 1
-    nxt = logits.argmax(-1, keepdim=True)
     pos = torch.tensor([prompt], device=device)
-    step = lambda: model.forward(nxt, pos, prompt + 1)
+    if sampling is None:
+        nxt = logits.argmax(-1, keepdim=True)
+        step = lambda: model.forward(nxt, pos, prompt + 1)
+    else:
+        uniform = torch.rand(batch, generator=gen, device=device)        # the same on every rank
+        nxt = mx.sample_logits(logits, uniform, **sampling)[:, None]
+        step = lambda: mx.sample_logits(model.forward(nxt, pos, prompt + 1), uniform, **sampling)
     full_ms = _time_graph(step, tokens)
     model.linears_only = True
     lin_ms = _time_graph(step, tokens)
@@ -217,7 +231,7 @@ def run(layers: int = 32, batch: int = 1, prompt: int = 2048, tokens: int = 32, 
         "prefill_ms": round(prefill_ms, 2), "prefill_tokens_per_s": round(batch * prompt / prefill_ms * 1e3, 1),
         "decode_ms_per_step": round(full_ms, 4), "decode_tokens_per_s": round(batch / full_ms * 1e3, 1),
         "mixfp4_linears_ms_per_step": round(lin_ms, 4), "mixfp4_linear_time_fraction": round(lin_ms / full_ms, 3),
-        "peer_wait_status": status,
+        "peer_wait_status": status, "head": head, "sampling": sampling,
     }
 
 
@@ -229,13 +243,19 @@ def main() -> None:
     ap.add_argument("--prompt", type=int, default=2048)
     ap.add_argument("--tokens", type=int, default=32)
     ap.add_argument("--tp", type=int, default=1, help="tensor-parallel degree (launch with torch.distributed.run)")
+    ap.add_argument("--head", choices=["bf16", "fp8"], default="bf16", help="precision of the output head")
+    ap.add_argument("--temperature", type=float, help="draw the tokens (0: the largest logit) instead of taking the argmax outside the step")
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
     args = ap.parse_args()
+    sampling = None if args.temperature is None else {"temperature": args.temperature, "top_k": args.top_k, "top_p": args.top_p, "min_p": args.min_p}
     local = int(os.environ.get("LOCAL_RANK", "0"))
     torch.cuda.set_device(local)
     if args.tp > 1:
         os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
         dist.init_process_group("nccl", device_id=torch.device("cuda", local))
-    result = run(args.layers, args.batch, args.prompt, args.tokens, tp=args.tp)
+    result = run(args.layers, args.batch, args.prompt, args.tokens, tp=args.tp, head=args.head, sampling=sampling)
     if args.tp == 1 or dist.get_rank() == 0:
         print(json.dumps(result))
     if args.tp > 1:

@@ -222,6 +222,87 @@ def test_module_keeps_its_format():
     assert torch.equal(other(x), layer(x))
 
 
+def test_operands_rewritten_just_before_the_call():
+    """The product starts under the tail of the kernel before it: whatever that writes, it is read as written."""
+    k, n = 2048, 1500
+    ws = [mx.quantize_fp8_weight(_data(n, k, torch.bfloat16, s)) for s in (1, 2)]
+    held = mx.FP8Weight.from_tensors(ws[0].codes.clone(), ws[0].scales.clone())
+    for m in (1, 20, 200, 1000):
+        xs = [_data(m, k, torch.bfloat16, 10 + s) for s in (1, 2)]
+        want = [mx.fp8_linear(x, w) for x, w in zip(xs, ws)]
+        qs = [mx.quantize_fp8_activations(x) for x in xs]
+        x, got = xs[0].clone(), []
+        q = mx.FP8Activations.from_tensors(qs[0].codes.clone(), qs[0].scales.clone())
+        torch.cuda.synchronize()
+        for i in range(12):
+            held.codes.copy_(ws[i % 2].codes)
+            held.scales.copy_(ws[i % 2].scales)
+            x.copy_(xs[i % 2])
+            got.append(mx.fp8_linear(x, held))
+            q.codes.copy_(qs[i % 2].codes)
+            q.scales.copy_(qs[i % 2].scales)
+            got.append(mx.fp8_linear(q, held))
+        for i, y in enumerate(got):
+            assert torch.equal(y, want[i // 2 % 2]), (m, i)
+
+
+def test_a_weight_past_2_31_elements():
+    n, k = 530000, 4096
+    weight = mx.quantize_fp8_weight(torch.ones((n, k), dtype=torch.bfloat16, device="cuda").mul_(torch.arange(n, device="cuda").remainder_(7)[:, None] + 1))
+    for m in (1, 70):
+        x = _data(m, k, torch.bfloat16, m, spread=False)
+        y = mx.fp8_linear(x, weight)
+        tail = mx.FP8Weight.from_tensors(weight.codes[n - 208:], weight.scales[-2:])      # 530000 = 4140 * 128 + 80
+        part = mx.fp8_linear(x, mx.quantize_fp8_weight(weight.dequantize(torch.bfloat16)[n - 80:]))
+        q = mx.quantize_fp8_activations(x)
+        _check_product(y[:, n - 80:], _expand(q.codes, q.scales, 1), _expand(weight.codes[n - 80:], weight.scales[-1:], 128), torch.bfloat16)
+        assert part.shape == (m, 80) and tail.n == 208
+
+
+def test_two_streams_at_once():
+    weight = mx.quantize_fp8_weight(_data(3000, 1024, torch.bfloat16, 1))
+    xs = [_data(m, 1024, torch.bfloat16, m) for m in (3, 50, 130, 600)]
+    want = [mx.fp8_linear(x, weight) for x in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in xs], [[] for _ in xs]
+    for _ in range(10):
+        for x, st, out in zip(xs, streams, got):
+            with torch.cuda.stream(st):
+                out.append(mx.fp8_linear(x, weight))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for out, w in zip(got, want) for y in out) and mx.gemm_status() == 0
+
+
+def test_converted_model_and_checkpoint(tmp_path):
+    class Tiny(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.up_proj, self.down_proj = torch.nn.Linear(256, 384, bias=False), torch.nn.Linear(384, 256)
+            self.lm_head = torch.nn.Linear(256, 1000, bias=False)
+
+        def forward(self, x):
+            return self.lm_head(self.down_proj(torch.relu(self.up_proj(x))))
+
+    torch.manual_seed(0)
+    model = Tiny().to("cuda", torch.bfloat16)
+    dense = {n: m.weight.detach().clone() for n, m in model.named_modules() if isinstance(m, torch.nn.Linear)}
+    bias = model.down_proj.bias.detach().clone()
+    rows = mx.quantize_model_weights(model, "oracle16", per_module_mode={"down_proj": "fp8", "lm_head": "fp8"})
+    assert [(r["module_name"], r["format_granularity"]) for r in rows] == [("up_proj", "oracle16"), ("down_proj", "fp8"), ("lm_head", "fp8")]
+    assert isinstance(model.up_proj, mx.MixFP4Linear) and isinstance(model.lm_head, mx.FP8Linear)
+    x = _data(5, 256, torch.bfloat16, 3, spread=False)
+    y = model(x)
+    h = torch.relu(model.up_proj(x))
+    h = mx.fp8_linear(h, mx.quantize_fp8_weight(dense["down_proj"]), bias=bias)
+    assert torch.equal(y, mx.fp8_linear(h, mx.quantize_fp8_weight(dense["lm_head"])))
+    path = str(tmp_path / "packed.pt")
+    mx.save_packed(model, path)
+    torch.manual_seed(1)
+    other = Tiny().to("cuda", torch.bfloat16)
+    assert set(mx.load_packed(other, path)) == {"up_proj", "down_proj", "lm_head"}
+    assert torch.equal(other(x), y)
+
+
 def test_refusals():
     x, weight = _data(4, 256, torch.bfloat16, 1), mx.quantize_fp8_weight(_data(64, 256, torch.bfloat16, 2))
     with pytest.raises(ValueError):

@@ -1,0 +1,101 @@
+"""What of the block-scaled FP8 linear and of token sampling needs no GPU: refusals, at the C boundary before any CUDA call and in
+Python, and the converter's choice of layers."""
+
+import ctypes
+
+import pytest
+import torch
+
+import mixfp4_b200 as mx
+from mixfp4_b200 import _native as nat
+
+ONE = ctypes.c_void_p(64)       # never dereferenced: validation fails first
+ODD = ctypes.c_void_p(66)
+
+
+def _with(args, **changed):
+    args = list(args)
+    for at, value in changed.items():
+        args[int(at[1:])] = value
+    return args
+
+
+def test_sizes():
+    h = nat.lib()
+    assert [h.mixfp4_fp8_scale_rows(m) for m in (-1, 0, 1, 128, 129)] == [0, 0, 128, 128, 256]
+    assert h.mixfp4_fp8_workspace_bytes(1, 4096) == 0                       # quantized by the product itself
+    assert h.mixfp4_fp8_workspace_bytes(100, 300) == 100 * 384 + 128 * 3 * 4
+    assert h.mixfp4_fp8_workspace_bytes(0, 300) == 0 and h.mixfp4_sample_max_vocab() == 524160
+
+
+def test_quantizers_refuse():
+    h = nat.lib()
+    rows = (ONE, nat.BF16, 4, 256, 256, ONE, 256, ONE, 128, None)
+    for changed, status in (({"a0": None}, -1), ({"a5": None}, -1), ({"a7": None}, -1), ({"a1": 7}, -4), ({"a2": 0}, -2), ({"a3": 0}, -2),
+                            ({"a4": 255}, -2), ({"a6": 240}, -2), ({"a8": 127}, -2), ({"a5": ODD}, -3), ({"a6": 264}, -3), ({"a7": ODD}, -3),
+                            ({"a8": 130}, -3), ({"a3": 1 << 40, "a4": 1 << 40, "a6": 1 << 41}, -2)):
+        assert h.mixfp4_fp8_quantize_rows(*_with(rows, **changed)) == status, changed
+    tiles = (ONE, nat.BF16, 4, 256, 256, ONE, 256, ONE, None)
+    for changed, status in (({"a0": None}, -1), ({"a7": None}, -1), ({"a1": -1}, -4), ({"a2": -3}, -2), ({"a4": 128}, -2), ({"a6": 128}, -2),
+                            ({"a6": 264}, -3), ({"a5": ODD}, -3), ({"a7": ODD}, -3)):
+        assert h.mixfp4_fp8_quantize_tiles(*_with(tiles, **changed)) == status, changed
+    dequant = (ONE, 256, ONE, 2, 1, 128, 4, 256, ONE, nat.BF16, 256, None)
+    for changed, status in (({"a0": None}, -1), ({"a8": None}, -1), ({"a5": 64}, -5), ({"a6": 0}, -2), ({"a1": 255}, -2), ({"a10": 255}, -2),
+                            ({"a3": -1}, -2), ({"a9": 9}, -4)):
+        assert h.mixfp4_fp8_dequant(*_with(dequant, **changed)) == status, changed
+
+
+def test_products_refuse():
+    h = nat.lib()
+    gemm = (ONE, 256, ONE, 128, ONE, 256, ONE, 4, 64, 256, ONE, nat.BF16, 64, None, None)
+    for changed, status in (({"a0": None}, -1), ({"a2": None}, -1), ({"a4": None}, -1), ({"a6": None}, -1), ({"a10": None}, -1), ({"a1": 255}, -2),
+                            ({"a3": 4}, -2), ({"a5": 128}, -2), ({"a7": 0}, -2), ({"a8": 0}, -2), ({"a9": 0}, -2), ({"a12": 63}, -2), ({"a11": 5}, -4),
+                            ({"a0": ODD}, -3), ({"a1": 264}, -3), ({"a4": ODD}, -3), ({"a5": 264}, -3), ({"a6": ODD}, -3), ({"a2": ODD}, -3),
+                            ({"a7": 1 << 31}, -2)):
+        assert h.mixfp4_fp8_gemm(*_with(gemm, **changed)) == status, changed
+    linear = (ONE, nat.BF16, 100, 300, ONE, 304, ONE, 64, 300, ONE, nat.F32, 64, ONE, 1 << 20, None, None)
+    for changed, status in (({"a0": None}, -1), ({"a1": 7}, -4), ({"a3": 299}, -2), ({"a4": None}, -1), ({"a5": 300}, -3), ({"a9": None}, -1),
+                            ({"a12": None}, -7), ({"a13": 1000}, -7), ({"a12": ODD}, -3), ({"a10": 7}, -4)):
+        assert h.mixfp4_fp8_linear(*_with(linear, **changed)) == status, changed
+    few = _with(linear, a2=1, a12=None, a13=0)               # no workspace, but the same checks
+    for changed, status in (({"a0": None}, -1), ({"a1": 7}, -4), ({"a3": 299}, -2), ({"a5": 300}, -3)):
+        assert h.mixfp4_fp8_linear(*_with(few, **changed)) == status, changed
+
+
+def test_sampling_refuses():
+    h = nat.lib()
+    args = (ONE, nat.F32, 2, 100, 100, ONE, None, 1.0, None, 0, None, 1.0, None, 0.0, ONE, None, None)
+    for changed, status in (({"a0": None}, -1), ({"a5": None}, -1), ({"a14": None}, -1), ({"a2": 0}, -2), ({"a3": 0}, -2), ({"a4": 99}, -2),
+                            ({"a3": 600000, "a4": 600000}, -10), ({"a1": 4}, -4), ({"a0": ODD}, -3), ({"a5": ODD}, -3), ({"a14": ODD}, -3),
+                            ({"a2": 1 << 31}, -2)):
+        assert h.mixfp4_sample(*_with(args, **changed)) == status, changed
+
+
+def test_python_refusals():
+    x = torch.zeros((2, 8))
+    for call in (lambda: mx.quantize_fp8_weight(x), lambda: mx.quantize_fp8_activations(x), lambda: mx.sample_logits(x, torch.zeros(2))):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+    with pytest.raises(ValueError):
+        mx.quantize_fp8_weight(torch.zeros(8))
+    codes, scales = torch.zeros((200, 300), dtype=torch.uint8), torch.ones((2, 3))
+    weight = mx.FP8Weight.from_tensors(codes, scales)        # a container may live on the host
+    assert weight.codes.shape == (200, 300) and weight.codes.stride(0) == 384 and weight.nbytes() == 200 * 300 + 24
+    for bad in ((codes, scales[:1]), (codes[0], scales), (codes[:0], scales)):
+        with pytest.raises(ValueError):
+            mx.FP8Weight.from_tensors(*bad)
+    for bad in ((codes.float(), scales), (codes, scales.half())):
+        with pytest.raises(TypeError):
+            mx.FP8Weight.from_tensors(*bad)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        mx.fp8_linear(torch.zeros((2, 300)), weight)
+    with pytest.raises(ValueError):
+        mx.fp8_linear(torch.zeros((2, 299)), weight)
+
+
+def test_converter_refuses_names_that_are_no_linear():
+    model = torch.nn.Sequential(torch.nn.Linear(16, 16), torch.nn.ReLU())
+    for name in ("1", "missing"):
+        with pytest.raises(KeyError):
+            mx.quantize_model_weights(model, "bf16", per_module_mode={name: "fp8"})
+    assert mx.quantize_model_weights(model, "bf16") == []

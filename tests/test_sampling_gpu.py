@@ -159,6 +159,38 @@ def test_head_and_sampling_together():
     _check(mx.fp8_linear(h, head), u, temperature=0.8, top_k=40, top_p=0.95)
 
 
+def test_logits_rewritten_just_before_the_call():
+    a, u = _logits(3, 6000, torch.bfloat16, 1)
+    b, _ = _logits(3, 6000, torch.bfloat16, 2)
+    want = [mx.sample_logits(x, u, top_k=30, top_p=0.9) for x in (a, b)]
+    x, got = a.clone(), []
+    for i in range(20):
+        x.copy_((a, b)[i % 2])
+        got.append(mx.sample_logits(x, u, top_k=30, top_p=0.9))
+    assert all(torch.equal(t, want[i % 2]) for i, t in enumerate(got))
+
+
+def test_logits_past_2_31_elements():
+    rows, vocab = 4400, 500000
+    x = torch.zeros((rows, vocab), dtype=torch.bfloat16, device="cuda")
+    at = torch.arange(rows, device="cuda") * 113 % vocab
+    x.scatter_(1, at[:, None], 50.0)
+    u = torch.full((rows,), 0.5, device="cuda")
+    for settings in (dict(top_k=5), dict(top_p=0.9), dict(temperature=0.0)):
+        assert torch.equal(mx.sample_logits(x, u, **settings), at)
+
+
+def test_decoder_draws_its_tokens():
+    """The harness with an FP8 head, sampling within the captured decode step."""
+    from mixfp4_b200.llama_decode import run
+
+    keep = {}
+    settings = {"temperature": 0.8, "top_k": 50, "top_p": 0.95, "min_p": 0.0}
+    got = run(layers=1, batch=2, prompt=32, tokens=2, keep=keep, head="fp8", sampling=settings)
+    assert got["head"] == "fp8" and got["sampling"] == settings and got["decode_ms_per_step"] > 0
+    assert run(layers=1, batch=2, prompt=32, tokens=2, weights=keep["weights"])["sampling"] is None
+
+
 def test_refusals():
     x, u = _logits(4, 100, torch.float32, 1)
     for bad in (dict(temperature=-1.0), dict(top_p=1.5), dict(min_p=-0.1), dict(top_p=torch.ones(3, device="cuda"))):
