@@ -66,8 +66,8 @@ def sample_logits(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     k, k_all = _setting(top_k, "top_k", torch.int32, rows, device, -1, 2 ** 31 - 1)
     p, p_all = _setting(top_p, "top_p", torch.float32, rows, device, 0.0, 1.0)
     f, f_all = _setting(min_p, "min_p", torch.float32, rows, device, 0.0, 1.0)
-    token = torch.empty(lead, dtype=torch.int64, device=device)
-    logprob = torch.empty(lead, dtype=torch.float32, device=device) if return_logprob else None
+    token = torch.empty_strided((rows,), (1,), dtype=torch.int64, device=device)      # a microsecond less than torch.empty
+    logprob = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=device) if return_logprob else None
     if rows:
         stride = x.stride(0)
         if x.stride(1) != 1 and vocab > 1 or rows > 1 and stride < vocab:
@@ -79,4 +79,6 @@ def sample_logits(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
                                          nat.ptr(t), t_all, nat.ptr(k), k_all, nat.ptr(p), p_all, nat.ptr(f), f_all,
                                          token.data_ptr(), nat.ptr(logprob), nat.stream_ptr(device))
         nat.check("mixfp4_sample", st)
+    if len(lead) != 1:
+        token, logprob = token.reshape(lead), None if logprob is None else logprob.reshape(lead)
     return (token, logprob) if return_logprob else token
