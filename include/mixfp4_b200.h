@@ -396,7 +396,7 @@ MIXFP4_API int mixfp4_gemm_h128_static(const void* x, int64_t m, int64_t ldx,
  * mixfp4_fp8_quantize_rows: x [m, k] (any element type, row stride ldx) -> codes [m, ldq], zero from k to kpad, and scales
  *   [ceil(k/128)][lds], the scale of (row, block) at block * lds + row; lds >= mixfp4_fp8_scale_rows(m); rows m.. stay as they were.
  * mixfp4_fp8_quantize_tiles: w [n, k] -> codes [n, ldq] likewise, scales [ceil(n/128)][ceil(k/128)].
- * codes and scales 16-byte aligned (scales of tiles 4), ldq >= mixfp4_padded_k(k) and a multiple of 16, lds a multiple of 4.
+ * x, w and y lie on multiples of their element, here and below; codes and scales 16-byte aligned (scales of tiles 4), ldq >= mixfp4_padded_k(k) and a multiple of 16, lds a multiple of 4.
  * mixfp4_fp8_dequant: y[r, c] = code * scale[r / rows_per_scale * row_stride + c / 128 * block_stride], rounded once;
  *   rows_per_scale 1 or 128. */
 MIXFP4_API int64_t mixfp4_fp8_scale_rows(int64_t m);

@@ -16,6 +16,8 @@ inline bool fp8_quantizes_itself(int64_t m, int64_t k) {
     return m <= 64 && blocks <= 48 && m * blocks <= 128;
 }
 
+inline int fp8_elem_bytes(int dtype) { return dtype == MIXFP4_F32 ? 4 : 2; }
+
 // Arguments of mixfp4_fp8_quantize_rows, checked before any CUDA call; then the pass itself.
 int fp8_check_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx, const uint8_t* codes, int64_t ldq,
                    const float* scales, int64_t lds);

@@ -885,7 +885,7 @@ int check_product(const uint8_t* w, int64_t ldw, const float* sw, int64_t m, int
     if (!w || !sw || !y) return MIXFP4_E_NULL;
     if (out_dtype != MIXFP4_BF16 && out_dtype != MIXFP4_F16 && out_dtype != MIXFP4_F32) return MIXFP4_E_DTYPE;
     if (m <= 0 || n <= 0 || k <= 0 || m > kMaxSide || n > kMaxSide || k > kMaxSide || ldw < k || ldy < n) return MIXFP4_E_SHAPE;
-    if (!aligned(w, 16) || ldw % 16 != 0 || !aligned(sw, 4)) return MIXFP4_E_ALIGN;
+    if (!aligned(w, 16) || ldw % 16 != 0 || !aligned(sw, 4) || !aligned(y, fp8_elem_bytes(out_dtype))) return MIXFP4_E_ALIGN;
     return MIXFP4_OK;
 }
 
@@ -895,7 +895,7 @@ Fp8Args make_args(const float* sx, int64_t ldsx, const float* sw, int64_t m, int
     a.sx = sx; a.sw = sw; a.y = y; a.ldsx = ldsx; a.ldy = ldy;
     a.m = (int)m; a.n = (int)n; a.k = (int)k; a.blocks = (int)((k + kFp8Block - 1) / kFp8Block);
     a.out_dtype = out_dtype; a.status = status;
-    a.y_vec = aligned(y, 32) && ldy * (out_dtype == MIXFP4_F32 ? 4 : 2) % 32 == 0;
+    a.y_vec = aligned(y, 32) && ldy * fp8_elem_bytes(out_dtype) % 32 == 0;
     return a;
 }
 
@@ -931,8 +931,9 @@ extern "C" int mixfp4_fp8_linear(const void* x, int dtype, int64_t m, int64_t ld
     if (fp8_quantizes_itself(m, k)) {
         if (dtype != MIXFP4_BF16 && dtype != MIXFP4_F16 && dtype != MIXFP4_F32) return MIXFP4_E_DTYPE;
         if (ldx < k) return MIXFP4_E_SHAPE;
+        if (!aligned(x, fp8_elem_bytes(dtype))) return MIXFP4_E_ALIGN;
         a.x = x; a.ldx = ldx; a.x_dtype = dtype;
-        a.x_vec = aligned(x, 16) && ldx * (dtype == MIXFP4_F32 ? 4 : 2) % 16 == 0;
+        a.x_vec = aligned(x, 16) && ldx * fp8_elem_bytes(dtype) % 16 == 0;
         return fp8_gemm(a, Fp8Problem{nullptr, 0, w, ldw, k, false, true}, st);
     }
     if (!workspace || workspace_bytes < mixfp4_fp8_workspace_bytes(m, k)) return MIXFP4_E_WORKSPACE;

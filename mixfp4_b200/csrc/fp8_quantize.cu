@@ -102,7 +102,6 @@ int by_type(int dtype, F&& f) {
         default: return MIXFP4_E_DTYPE;
     }
 }
-int elem_bytes(int dtype) { return dtype == MIXFP4_F32 ? 4 : 2; }
 constexpr int64_t kMaxSide = 0x7fffffff;          // a tensor map's coordinates are 32-bit
 
 }  // namespace
@@ -113,7 +112,8 @@ int fp8_check_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx, 
     if (dtype != MIXFP4_BF16 && dtype != MIXFP4_F16 && dtype != MIXFP4_F32) return MIXFP4_E_DTYPE;
     if (m <= 0 || k <= 0 || m > kMaxSide || k > kMaxSide - 128 || ldx < k || ldq < padded_k(k) || lds < fp8_scale_rows(m))
         return MIXFP4_E_SHAPE;
-    if (!aligned(codes, 16) || ldq % 16 != 0 || !aligned(scales, 16) || lds % 4 != 0) return MIXFP4_E_ALIGN;
+    if (!aligned(x, fp8_elem_bytes(dtype)) || !aligned(codes, 16) || ldq % 16 != 0 || !aligned(scales, 16) || lds % 4 != 0)
+        return MIXFP4_E_ALIGN;
     return MIXFP4_OK;
 }
 
@@ -158,8 +158,8 @@ extern "C" int mixfp4_fp8_quantize_tiles(const void* w, int dtype, int64_t n, in
     if (n <= 0 || k <= 0 || n > kMaxSide - 128 || k > kMaxSide - 128 || ldw < k || ldq < padded_k(k)) return MIXFP4_E_SHAPE;
     const int64_t tiles = (n + kFp8Block - 1) / kFp8Block * ((k + kFp8Block - 1) / kFp8Block);
     if (tiles > kMaxSide) return MIXFP4_E_SHAPE;
-    if (!aligned(codes, 16) || ldq % 16 != 0 || !aligned(scales, 4)) return MIXFP4_E_ALIGN;
-    const bool vec = aligned(w, 16) && ldw * elem_bytes(dtype) % 16 == 0;
+    if (!aligned(w, fp8_elem_bytes(dtype)) || !aligned(codes, 16) || ldq % 16 != 0 || !aligned(scales, 4)) return MIXFP4_E_ALIGN;
+    const bool vec = aligned(w, 16) && ldw * fp8_elem_bytes(dtype) % 16 == 0;
     return by_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
         fp8_tiles_kernel<T><<<(unsigned)tiles, kTileThreads, 0, static_cast<cudaStream_t>(stream)>>>(
@@ -175,6 +175,8 @@ extern "C" int mixfp4_fp8_dequant(const uint8_t* codes, int64_t ldq, const float
     if (rows_per_scale != 1 && rows_per_scale != kFp8Block) return MIXFP4_E_MODE;
     if (rows <= 0 || k <= 0 || rows > kMaxSide || k > kMaxSide || ldq < k || ldy < k || row_stride < 0 || block_stride < 0)
         return MIXFP4_E_SHAPE;
+    if (out_dtype != MIXFP4_BF16 && out_dtype != MIXFP4_F16 && out_dtype != MIXFP4_F32) return MIXFP4_E_DTYPE;
+    if (!aligned(scales, 4) || !aligned(y, fp8_elem_bytes(out_dtype))) return MIXFP4_E_ALIGN;
     return by_type(out_dtype, [&](auto t) -> int {
         using T = decltype(t);
         const int64_t ctas = (rows * ((k + 3) / 4) + 255) / 256;

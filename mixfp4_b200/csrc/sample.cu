@@ -720,7 +720,9 @@ extern "C" int mixfp4_sample(const void* logits, int dtype, int64_t rows, int64_
     if (vocab > kMaxVocab) return MIXFP4_E_TOO_LARGE;
     const int bytes = dtype == MIXFP4_F32 ? 4 : 2;
     if (dtype != MIXFP4_BF16 && dtype != MIXFP4_F16 && dtype != MIXFP4_F32) return MIXFP4_E_DTYPE;
-    if (!aligned(logits, bytes) || !aligned(uniform, 4) || !aligned(token, 8)) return MIXFP4_E_ALIGN;
+    if (!aligned(logits, bytes) || !aligned(uniform, 4) || !aligned(token, 8) || !aligned(temperature, 4) || !aligned(top_k, 4) ||
+        !aligned(top_p, 4) || !aligned(min_p, 4) || !aligned(logprob, 4))
+        return MIXFP4_E_ALIGN;
     SampleArgs a = {};
     a.logits = logits; a.ld = ld; a.vocab = (int)vocab; a.uniform = uniform;
     a.temperature = {temperature, temperature_all}; a.top_k = {top_k, top_k_all};

@@ -71,6 +71,23 @@ def test_sampling_refuses():
         assert h.mixfp4_sample(*_with(args, **changed)) == status, changed
 
 
+def test_pointers_off_their_element_are_refused():
+    h = nat.lib()
+    off2, off4 = ctypes.c_void_p(65), ctypes.c_void_p(66)
+    for dtype, off in ((nat.BF16, off2), (nat.F16, off2), (nat.F32, off4)):
+        assert h.mixfp4_fp8_quantize_rows(off, dtype, 4, 256, 256, ONE, 256, ONE, 128, None) == -3
+        assert h.mixfp4_fp8_quantize_tiles(off, dtype, 4, 256, 256, ONE, 256, ONE, None) == -3
+        assert h.mixfp4_fp8_dequant(ONE, 256, ONE, 2, 1, 128, 4, 256, off, dtype, 256, None) == -3
+        assert h.mixfp4_fp8_gemm(ONE, 256, ONE, 128, ONE, 256, ONE, 4, 64, 256, off, dtype, 64, None, None) == -3
+        for m in (1, 1000):                                  # quantized by the product, and ahead of it
+            assert h.mixfp4_fp8_linear(off, dtype, m, 256, ONE, 256, ONE, 64, 256, ONE, nat.F32, 64, ONE, 1 << 20, None, None) == -3
+            assert h.mixfp4_fp8_linear(ONE, nat.F32, m, 256, ONE, 256, ONE, 64, 256, off, dtype, 64, ONE, 1 << 20, None, None) == -3
+    assert h.mixfp4_fp8_dequant(ONE, 256, off4, 2, 1, 128, 4, 256, ONE, nat.BF16, 256, None) == -3
+    args = (ONE, nat.F32, 2, 100, 100, ONE, None, 1.0, None, 0, None, 1.0, None, 0.0, ONE, None, None)
+    for at in (0, 5, 6, 8, 10, 12, 15):
+        assert h.mixfp4_sample(*_with(args, **{f"a{at}": off4})) == -3, at
+
+
 def test_python_refusals():
     x = torch.zeros((2, 8))
     for call in (lambda: mx.quantize_fp8_weight(x), lambda: mx.quantize_fp8_activations(x), lambda: mx.sample_logits(x, torch.zeros(2))):
