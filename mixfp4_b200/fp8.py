@@ -11,6 +11,7 @@ counterpart of this format in it.  Inputs that are not finite make their block's
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -26,10 +27,15 @@ def _blocks(size: int) -> int:
     return -(-size // FP8_BLOCK)
 
 
+def _addressable(codes: torch.Tensor) -> bool:
+    """Rows that a tensor map can address: unit stride along K, each on 16 bytes."""
+    return codes.stride(1) == 1 and codes.stride(0) >= codes.shape[1] and codes.stride(0) % 16 == 0 and codes.data_ptr() % 16 == 0
+
+
 def _codes_for_kernels(codes: torch.Tensor) -> torch.Tensor:
     """The codes with rows that a tensor map can address (16-byte aligned); themselves where they are so already."""
     rows, k = codes.shape
-    if codes.stride(1) == 1 and codes.stride(0) >= k and codes.stride(0) % 16 == 0 and codes.data_ptr() % 16 == 0:
+    if _addressable(codes):
         return codes
     held = torch.empty((rows, _blocks(k) * FP8_BLOCK), dtype=codes.dtype, device=codes.device)[:, :k]
     held.copy_(codes)
@@ -41,7 +47,7 @@ def _check_parts(codes: torch.Tensor, scales: torch.Tensor, rows_per_scale: int)
         codes = codes.view(torch.float8_e4m3fn)
     if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
         raise TypeError("codes must be float8_e4m3fn (or its bytes), scales float32")
-    if codes.ndim != 2 or 0 in codes.shape:
+    if codes.ndim != 2 or codes.shape[1] == 0 or codes.shape[0] == 0 and rows_per_scale > 1:
         raise ValueError("codes must be a matrix with at least one row and column")
     want = (-(-codes.shape[0] // rows_per_scale), _blocks(codes.shape[1]))
     if tuple(scales.shape) != want:
@@ -53,12 +59,16 @@ def _check_parts(codes: torch.Tensor, scales: torch.Tensor, rows_per_scale: int)
 
 @dataclass
 class FP8Weight:
-    """A quantized [n, k] weight: codes float8_e4m3fn [n, k] with 16-byte aligned rows, scales float32 [ceil(n/128), ceil(k/128)]."""
+    """A quantized [n, k] weight: codes float8_e4m3fn [n, k] with 16-byte aligned rows, scales float32 [ceil(n/128), ceil(k/128)],
+    contiguous.  (`from_tensors` takes any strides and brings them there.)"""
 
     codes: torch.Tensor
     scales: torch.Tensor
 
     def __post_init__(self):
+        self.codes = _check_parts(self.codes, self.scales, FP8_BLOCK)
+        if not _addressable(self.codes) or not self.scales.is_contiguous():
+            raise ValueError("a weight's code rows are 16-byte aligned and its scales contiguous: FP8Weight.from_tensors makes them so")
         self.n, self.k = self.codes.shape
 
     @classmethod
@@ -84,12 +94,33 @@ class FP8Weight:
 @dataclass
 class FP8Activations:
     """Quantized rows: codes float8_e4m3fn [m, k]; scales float32 [m, ceil(k/128)], a view whose columns are contiguous and
-    padded to 128 rows (what the product fetches).  `shape` and `dtype` are the source's."""
+    padded to 128 rows (what the product fetches).  `shape` and `dtype` are the source's.  (`from_tensors` takes any strides
+    and brings them there.)"""
 
     codes: torch.Tensor
     scales: torch.Tensor
     shape: torch.Size
     dtype: torch.dtype
+
+    def __post_init__(self):
+        codes, scales = _check_parts(self.codes, self.scales, 1), self.scales
+        m, k = codes.shape
+        room, ld = _blocks(m) * FP8_BLOCK, scales.stride(1)
+        held = scales.untyped_storage().nbytes() // 4 - scales.storage_offset()
+        if (not _addressable(codes) or m > 1 and scales.stride(0) != 1 or m and (ld < room or ld % 4 != 0 or scales.data_ptr() % 16 != 0
+                                                                                or held < (scales.shape[1] - 1) * ld + room)):
+            raise ValueError("code rows are 16-byte aligned, and columns of scales have room for 128 rows: FP8Activations.from_tensors "
+                             "makes them so")
+        if self.shape[-1] != k or math.prod(self.shape[:-1]) != m:
+            raise ValueError(f"codes {tuple(codes.shape)} are not rows of a tensor of shape {tuple(self.shape)}")
+        self.codes = codes
+
+    @classmethod
+    def _made(cls, codes, scales, shape, dtype) -> "FP8Activations":
+        """Parts that this module made itself: nothing to check."""
+        q = object.__new__(cls)
+        q.codes, q.scales, q.shape, q.dtype = codes, scales, shape, dtype
+        return q
 
     @classmethod
     def from_tensors(cls, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> "FP8Activations":
@@ -155,7 +186,7 @@ def quantize_fp8_activations(x: torch.Tensor) -> FP8Activations:
                                                     codes.stride(0), scales.data_ptr(), _blocks(m) * FP8_BLOCK,
                                                     nat.stream_ptr(x.device))
         nat.check("mixfp4_fp8_quantize_rows", st)
-    return FP8Activations(codes if codes.shape[1] == k else codes[:, :k], scales, x.shape, x.dtype)
+    return FP8Activations._made(codes if codes.shape[1] == k else codes[:, :k], scales, x.shape, x.dtype)
 
 
 def dequantize_fp8(q: FP8Weight | FP8Activations, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -221,6 +252,7 @@ class FP8Linear(nn.Module):
     def __init__(self, weight: FP8Weight, bias: torch.Tensor | None = None):
         super().__init__()
         self.in_features, self.out_features = weight.k, weight.n
+        self._weight = None
         self.register_buffer("codes", weight.codes)
         self.register_buffer("scales", weight.scales)
         self.bias = None if bias is None else nn.Parameter(bias.detach().clone(), requires_grad=False)
@@ -235,7 +267,12 @@ class FP8Linear(nn.Module):
 
     @property
     def weight_fp8(self) -> FP8Weight:
-        return FP8Weight(self.codes, self.scales)
+        """The layer's buffers as a weight; checked again when they are others (`load_state_dict(assign=True)`)."""
+        held = self._weight
+        if held is None or held.codes is not self.codes or held.scales is not self.scales:
+            held = self._weight = FP8Weight.from_tensors(self.codes, self.scales)
+            self.codes, self.scales = held.codes, held.scales
+        return held
 
     @classmethod
     @torch.no_grad()

@@ -1,6 +1,7 @@
 """What of the block-scaled FP8 linear and of token sampling needs no GPU: refusals, at the C boundary before any CUDA call and in
 Python, and the converter's choice of layers."""
 
+import copy
 import ctypes
 
 import pytest
@@ -108,6 +109,41 @@ def test_python_refusals():
         mx.fp8_linear(torch.zeros((2, 300)), weight)
     with pytest.raises(ValueError):
         mx.fp8_linear(torch.zeros((2, 299)), weight)
+
+
+def test_parts_that_the_kernels_cannot_read_are_refused():
+    codes, scales = torch.zeros((200, 384), dtype=torch.float8_e4m3fn), torch.ones((2, 3))
+    assert mx.FP8Weight(codes, scales).n == 200
+    for bad in ((codes[:, ::2], scales[:, :2]), (codes, torch.ones((3, 2)).t()), (codes, torch.ones((2, 6))[:, ::2]), (codes, scales[:, :2]),
+                (codes.view(torch.uint8)[:, 1:].view(torch.float8_e4m3fn), scales), (codes[:, :300].contiguous(), scales)):
+        with pytest.raises(ValueError):
+            mx.FP8Weight(*bad)
+        if bad[1].shape == (-(-bad[0].shape[0] // 128), -(-bad[0].shape[1] // 128)):
+            assert mx.FP8Weight.from_tensors(*bad).codes.stride(0) % 16 == 0
+    rows = torch.zeros((5, 384), dtype=torch.float8_e4m3fn)
+    good = mx.FP8Activations.from_tensors(rows, torch.ones((5, 3)))
+    shape, kind = torch.Size((5, 384)), torch.bfloat16
+    assert mx.FP8Activations(rows, good.scales, shape, kind).shape == shape
+    assert mx.FP8Activations(rows, good.scales, torch.Size((1, 5, 384)), kind).codes.shape == (5, 384)
+    wide = torch.ones((3, 256)).t()
+    for bad in ((rows, torch.ones((5, 3)), shape), (rows, wide[:10:2], shape), (rows, torch.ones((3, 130)).t()[:5], shape),
+                (rows, wide[1:6], shape), (rows, wide[252:], shape), (rows, good.scales, torch.Size((6, 384))), (rows, good.scales.double(), shape),
+                (rows, good.scales, torch.Size((5, 300))), (rows[:4], good.scales, shape), (rows[:, ::2], good.scales[:, :2], shape)):
+        with pytest.raises((ValueError, TypeError)):
+            mx.FP8Activations(*bad, kind)
+    assert mx.FP8Activations.from_tensors(rows[:0], torch.ones((0, 3))).shape == (0, 384)
+
+
+def test_a_layer_follows_its_buffers():
+    layer = mx.FP8Linear(mx.FP8Weight.from_tensors(torch.zeros((200, 300), dtype=torch.uint8), torch.ones((2, 3))))
+    weight = layer.weight_fp8
+    assert layer.weight_fp8 is weight and copy.deepcopy(layer).weight_fp8 is not weight
+    packed = torch.ones((200, 300), dtype=torch.uint8).view(torch.float8_e4m3fn)             # rows off their 16 bytes
+    layer.load_state_dict({"codes": packed, "scales": torch.full((2, 3), 2.0)}, assign=True)
+    assert layer.weight_fp8 is not weight and layer.weight_fp8.codes.stride(0) == 384
+    assert torch.equal(layer.weight_fp8.codes.view(torch.uint8), packed.view(torch.uint8)) and (layer.scales == 2).all()
+    layer.half()
+    assert layer.codes.dtype == torch.float8_e4m3fn and layer.scales.dtype == torch.float32
 
 
 def test_converter_refuses_names_that_are_no_linear():
