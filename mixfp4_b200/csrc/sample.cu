@@ -373,7 +373,7 @@ struct Sampler {
         ahead = (uint32_t)join(ahead);
         bool kept = i < n && ahead < k;
         const u64 of_k = block_sum(kept && part == 0 ? w : 0);
-        kept = kept && (p >= 1.0 || mass < share_of(p, of_k)) && w >= lowest;
+        kept = kept && (!(p < 1.0) || mass < share_of(p, of_k)) && w >= lowest;
         if (part == 0 && i < n) s.few_weight[i] = kept ? w : 0;
         const u64 total = block_sum(kept && part == 0 ? w : 0), goal = target_of(u, total);
         u64 at = 0;
@@ -524,7 +524,8 @@ struct Sampler {
                     bin = b;
                     const float width = 1.0f / bin_scale;
                     const float x_hi = largest - (float)bin * width * 0.9999f, x_lo = largest - ((float)bin + 1.0f) * width * 1.0001f;
-                    hi = Row<T>::key(bin == 0 ? largest : fminf(x_hi + fabsf(largest) * 1e-6f, largest));
+                    // (an edge that overflows bounds nothing: differences and temperatures near the largest float)
+                    hi = Row<T>::key(bin == 0 || !(x_hi > -FLT_MAX) ? largest : fminf(x_hi + fabsf(largest) * 1e-6f, largest));
                     lo = isinf(largest) ? hi : Row<T>::key(cut.value);
                     if (bin < (uint32_t)kBins - 1) lo = max(lo, Row<T>::key(x_lo - fabsf(largest) * 1e-6f));
                 } else {

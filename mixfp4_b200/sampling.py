@@ -42,7 +42,7 @@ def sample_logits(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     temperature, top_k, top_p, min_p: a number, or a tensor with one value for each row (fp32; top_k int32) on the logits'
     device.  temperature 0 takes the first of the largest logits; top_k <= 0 or >= V, top_p 1 and min_p 0 filter nothing;
     top_p 0 keeps the largest alone.  Tensor values are not read by the host: a temperature that is not above zero counts
-    as 0, a top_p or min_p outside [0, 1] as the nearer end, a uniform outside [0, 1) likewise.
+    as 0, a top_p or min_p outside [0, 1] as the nearer end, a uniform outside [0, 1) likewise; NaN as no filter, uniform NaN as 0.
     A logit of -inf or NaN is never chosen; +inf takes all the weight.  A row without a logit above -inf gives the token -1.
     return_logprob: also the natural logarithm of the token's share of the kept weights, fp32 [...] (-inf beside -1).
 
@@ -63,7 +63,7 @@ def sample_logits(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     if uniform.device != device:
         raise ValueError(f"uniform is on {uniform.device}, the logits on {device}")
     t, t_all = _setting(temperature, "temperature", torch.float32, rows, device, 0.0, 3.0e38)
-    k, k_all = _setting(top_k, "top_k", torch.int32, rows, device, -1, 2 ** 31 - 1)
+    k, k_all = _setting(top_k, "top_k", torch.int32, rows, device, -(2 ** 31), 2 ** 31 - 1)
     p, p_all = _setting(top_p, "top_p", torch.float32, rows, device, 0.0, 1.0)
     f, f_all = _setting(min_p, "min_p", torch.float32, rows, device, 0.0, 1.0)
     token = torch.empty_strided((rows,), (1,), dtype=torch.int64, device=device)      # a microsecond less than torch.empty

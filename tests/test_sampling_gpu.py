@@ -207,3 +207,27 @@ def test_refusals():
         mx.sample_logits(x.double(), u)
     with pytest.raises(mx._native.MixFP4Error):
         mx.sample_logits(torch.zeros((1, 600000), device="cuda"), u[:1])
+
+
+def test_settings_that_are_nan_filter_nothing():
+    rows, nan = 6, torch.full((6,), math.nan, device="cuda")
+    x, u = _logits(rows, 5000, torch.float32, 41)
+    for k in (0, 40, 2000):                                 # no cut by count, a few candidates, many
+        plain = mx.sample_logits(x, u, top_k=k, return_logprob=True)
+        for settings in (dict(top_p=nan), dict(min_p=nan), dict(top_p=nan, min_p=nan)):
+            got = mx.sample_logits(x, u, top_k=k, return_logprob=True, **settings)
+            assert torch.equal(got[0], plain[0]) and torch.equal(got[1], plain[1]), (k, settings)
+    assert torch.equal(mx.sample_logits(x, u, temperature=nan), x.argmax(-1))
+    assert torch.equal(mx.sample_logits(x, nan), mx.sample_logits(x, torch.zeros_like(u)))
+    assert torch.equal(mx.sample_logits(x, u, top_k=-7), mx.sample_logits(x, u))
+
+
+@pytest.mark.parametrize("temperature", [1e-40, 1e-30, 1e30, 1e38, 3e38])
+def test_values_and_temperatures_near_the_ends_of_fp32(temperature):
+    """Differences of logits that overflow, and a width of the bins that does."""
+    g = torch.Generator().manual_seed(43)
+    for scale in (3e38, 1e38, 1e-38):
+        x = (scale * (2 * torch.rand((4, 3001), generator=g) - 1)).cuda()
+        u = torch.rand(4, generator=g).cuda()
+        for settings in (dict(), dict(top_k=700), dict(top_p=0.6), dict(top_k=2000, top_p=0.99)):
+            _check(x, u, temperature=temperature, **settings)
