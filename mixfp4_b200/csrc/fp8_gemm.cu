@@ -43,7 +43,7 @@ struct Fp8Args {
     int m, n, k, blocks;
     int x_tiles, items, cluster, stages, out_dtype;
     bool early_weights;                  // the kernel before writes x and nothing else of this one's: weights are asked for ahead of it
-    bool y_vec;                          // rows of y are 32-byte aligned
+    bool y_vec;                          // rows of y are whole 32-byte sectors
     int* status;
 };
 
@@ -62,11 +62,16 @@ struct Fp8Cfg {
     static constexpr uint32_t kPitch = kCols + 4;                       // floats of a lane in the exchange: lanes 16 bytes apart in the banks
 };
 
+// Rows of y that are off their sectors leave through a patch of 32 rows x kPatchCols columns a warp, so that a store's lanes are
+// neighbouring columns.
+constexpr int kPatchCols = 16, kPatchPitch = kPatchCols + 1;
+constexpr uint32_t kPatchBytes = 32 * kPatchPitch * 4;
+
 struct Fp8Layout {
-    uint32_t own, own_scales, scales, exchange, bars, misc, bytes;
+    uint32_t own, own_scales, scales, exchange, patches, bars, misc, bytes;
 };
 template <int kCols, bool kSwap, bool kOwn>
-__host__ __device__ inline Fp8Layout fp8_layout(int stages, int cluster, int blocks) {
+__host__ __device__ inline Fp8Layout fp8_layout(int stages, int cluster, int blocks, bool y_vec) {
     using C = Fp8Cfg<kCols, kSwap, kOwn>;
     const uint32_t run = kOwn ? (uint32_t)((blocks + cluster - 1) / cluster) : 0u;
     Fp8Layout l;
@@ -74,7 +79,8 @@ __host__ __device__ inline Fp8Layout fp8_layout(int stages, int cluster, int blo
     l.own_scales = l.own + run * C::kBBytes;
     l.scales = l.own_scales + run * kCols * 4u;
     l.exchange = l.scales + (uint32_t)stages * C::kScales * 4u;
-    l.bars = l.exchange + (cluster > 1 ? 128u * C::kPitch * 4u : 0u);
+    l.patches = l.exchange + (cluster > 1 ? 128u * C::kPitch * 4u : 0u);
+    l.bars = l.patches + (kSwap || cluster > 1 || y_vec ? 0u : C::kEpi * kPatchBytes);
     l.misc = l.bars + (2 * kMaxStages + 2 * 4 + 3) * 8;
     l.bytes = (l.misc + 16 + 1024 + 7) & ~7u;                           // + alignment slack
     return l;
@@ -203,18 +209,35 @@ __device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                  ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
-// kN consecutive columns of a row, a sector at a time where the whole run is inside and aligned.
+// kN consecutive columns of this lane's row, row0 + lane, by a whole warp.  A sector at a time where rows of y are whole sectors;
+// otherwise through the warp's patch (4096 x 4099 x 4096 bf16: 98 us, 4096 x 1000 x 4096: 27 us; each thread storing its row's
+// columns one by one, 32 sectors an instruction: 231 us and 61 us).
 template <int kN>
-__device__ __forceinline__ void store_run(const Fp8Args& a, int64_t row, int64_t col, const float (&v)[kN]) {
-    static_assert(kN % 16 == 0, "a run is stored in sectors");
-    if (!a.y_vec || col + kN > a.n) {
+__device__ __forceinline__ void store_run(const Fp8Args& a, int64_t row0, int64_t col, const float (&v)[kN], float* patch) {
+    static_assert(kN % 16 == 0 && kPatchCols == 16, "a run is stored in sectors");
+    const int lane = threadIdx.x & 31;
+    const int64_t row = row0 + lane;
+    if (!a.y_vec) {
 #pragma unroll
-        for (int j = 0; j < kN; ++j)
-            if (col + j < a.n) store_one(a, row, col + j, v[j]);
+        for (int c = 0; c < kN; c += kPatchCols) {
+#pragma unroll
+            for (int j = 0; j < kPatchCols; ++j) patch[lane * kPatchPitch + j] = v[c + j];
+            __syncwarp();
+            const int j = lane % kPatchCols;
+            if (col + c + j < a.n) {
+#pragma unroll 8
+                for (int i = lane / kPatchCols; i < 32; i += 32 / kPatchCols)
+                    if (row0 + i < a.m) store_one(a, row0 + i, col + c + j, patch[i * kPatchPitch + j]);
+            }
+            __syncwarp();
+        }
+    } else if (row >= a.m) {
+        return;
     } else if (a.out_dtype == MIXFP4_F32) {
         float* p = static_cast<float*>(a.y) + row * a.ldy + col;
 #pragma unroll
         for (int j = 0; j < kN; j += 8) {
+            if (col + j >= a.n) break;
             uint32_t w[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[j + i]);
@@ -224,6 +247,7 @@ __device__ __forceinline__ void store_run(const Fp8Args& a, int64_t row, int64_t
         __half* p = static_cast<__half*>(a.y) + row * a.ldy + col;
 #pragma unroll
         for (int j = 0; j < kN; j += 16) {
+            if (col + j >= a.n) break;
             uint32_t w[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -323,7 +347,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;        // the same offset in every CTA of the cluster
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    const Fp8Layout L = fp8_layout<kCols, kSwap, kOwn>(a.stages, a.cluster, a.blocks);
+    const Fp8Layout L = fp8_layout<kCols, kSwap, kOwn>(a.stages, a.cluster, a.blocks, a.y_vec);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int rank = (int)cluster_ctarank();
     auto full = [&](int s) { return base + L.bars + s * 8; };
@@ -482,8 +506,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                         for (int j = 0; j < C::kPer; ++j)
                             if (x0 + half * C::kPer + j < a.m) store_one(a, x0 + half * C::kPer + j, w0 + tl, acc[j]);
                     }
-                } else if (x0 + tl < a.m) {
-                    store_run<C::kPer>(a, x0 + tl, w0 + half * C::kPer, acc);
+                } else {
+                    store_run<C::kPer>(a, x0 + quad * 32, w0 + half * C::kPer, acc, reinterpret_cast<float*>(gen + L.patches + warp * kPatchBytes));
                 }
                 continue;
             }
@@ -543,7 +567,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 // both CTAs' bytes, its commits release stages and report buffers in both, its acc_empty counts both CTAs' epilogue warps.
 constexpr uint32_t kLeaderMask = 0xFEFFFFFFu;        // clears the CTA-rank bit of a shared::cluster address
 constexpr int kPairEpi = 8, kPairThreads = (kPairEpi + 4) * 32, kPairStages = 6, kPairBufs = 2;
-constexpr uint32_t kPairHalf = 128 * 128, kPairStage = 2 * kPairHalf, kPairBars = kPairStages * kPairStage;
+constexpr uint32_t kPairHalf = 128 * 128, kPairStage = 2 * kPairHalf, kPairPatches = kPairStages * kPairStage, kPairBars = kPairPatches + kPairEpi * kPatchBytes;
 constexpr uint32_t kPairMisc = kPairBars + (2 * kPairStages + 2 * kPairBufs) * 8, kPairBytes = kPairMisc + 16 + 1024;
 constexpr uint32_t kPairInstrDesc = (1u << 4) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
 
@@ -700,7 +724,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 });
                 if (++b == kPairBufs) { b = 0; bph ^= 1; }
             }
-            if (ok && row < a.m) store_run(a, row, w0, acc);
+            if (ok) store_run(a, row - lane, w0, acc, reinterpret_cast<float*>(gen + kPairPatches + warp * kPatchBytes));
         }
     }
     // Both CTAs stay until the pair is done: the leader's MMAs read the peer's shared memory, the peer arrives on its barriers.
@@ -851,11 +875,11 @@ template <int kCols, bool kSwap, bool kOwn>
 int launch_single(Fp8Args a, const Fp8Problem& p, const Fp8Choice& c, cudaStream_t st) {
     a.cluster = 1 << c.cluster_log;
     a.stages = kMaxStages;
-    while (fp8_layout<kCols, kSwap, kOwn>(a.stages, a.cluster, a.blocks).bytes > kSmemMax) --a.stages;
+    while (fp8_layout<kCols, kSwap, kOwn>(a.stages, a.cluster, a.blocks, a.y_vec).bytes > kSmemMax) --a.stages;
     const auto kernel = fp8_gemm_kernel<kCols, kSwap, kOwn>;
     constexpr int kX = kSwap ? kCols : 128, kW = kSwap ? 128 : kCols;
     return launch_fp8(a, p, c, kX, kW, kX, kW, reinterpret_cast<const void*>(kernel), Fp8Cfg<kCols, kSwap, kOwn>::kThreads,
-                      fp8_layout<kCols, kSwap, kOwn>(a.stages, a.cluster, a.blocks).bytes, st);
+                      fp8_layout<kCols, kSwap, kOwn>(a.stages, a.cluster, a.blocks, a.y_vec).bytes, st);
 }
 template <int kCols, bool kOwn>
 int few_rows(const Fp8Args& a, const Fp8Problem& p, cudaStream_t st) {
@@ -895,7 +919,7 @@ Fp8Args make_args(const float* sx, int64_t ldsx, const float* sw, int64_t m, int
     a.sx = sx; a.sw = sw; a.y = y; a.ldsx = ldsx; a.ldy = ldy;
     a.m = (int)m; a.n = (int)n; a.k = (int)k; a.blocks = (int)((k + kFp8Block - 1) / kFp8Block);
     a.out_dtype = out_dtype; a.status = status;
-    a.y_vec = aligned(y, 32) && ldy * fp8_elem_bytes(out_dtype) % 32 == 0;
+    a.y_vec = aligned(y, 32) && ldy * fp8_elem_bytes(out_dtype) % 32 == 0 && n * fp8_elem_bytes(out_dtype) % 32 == 0;
     return a;
 }
 

@@ -317,3 +317,24 @@ def test_refusals():
         mx.FP8Weight.from_tensors(weight.codes, weight.scales[:, :1])
     with pytest.raises(TypeError):
         mx.FP8Weight.from_tensors(weight.codes, weight.scales.half())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n", [(40, 2051), (500, 2051), (1100, 2051), (500, 2048), (1100, 2064)])
+def test_rows_of_y_at_any_offset_and_stride(m, n, dtype):
+    """Few rows, one CTA a tile, CTA pairs: rows that are whole sectors and rows that are not; what lies between them stays."""
+    k = 640
+    x, w = _data(m, k, torch.bfloat16, 51), _data(n, k, torch.bfloat16, 52)
+    q, weight = mx.quantize_fp8_activations(x), mx.quantize_fp8_weight(w)
+    want = mx.fp8_linear(q, weight, out_dtype=dtype)
+    _check_product(want, _expand(q.codes, q.scales, 1), _expand(weight.codes, weight.scales, 128), dtype)
+    for offset, ldy in ((0, n), (1, n + 3), (0, -(-n // 32) * 32 + 32), (16, n + 1)):
+        held = torch.full((offset + m * ldy + 64,), 7.0, dtype=dtype, device="cuda")
+        status = nat.lib().mixfp4_fp8_gemm(q.codes.data_ptr(), q.codes.stride(0), q.scales.data_ptr(), q.scales.stride(1),
+                                           weight.codes.data_ptr(), weight.codes.stride(0), weight.scales.data_ptr(), m, n, k,
+                                           held[offset:].data_ptr(), nat.DTYPE_CODE[dtype], ldy, None,
+                                           torch.cuda.current_stream().cuda_stream)
+        assert status == 0
+        rows = held[offset: offset + m * ldy].view(m, ldy)
+        assert torch.equal(rows[:, :n], want), (offset, ldy)
+        assert (held[:offset] == 7).all() and (rows[:, n:] == 7).all() and (held[offset + m * ldy:] == 7).all()
