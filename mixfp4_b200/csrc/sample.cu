@@ -696,9 +696,17 @@ template <typename T>
 int sample(SampleArgs& a, int64_t rows, cudaStream_t st) {
     constexpr int kPer = 16 / sizeof(T);
     auto slice = [&](int ranks) { return ((int64_t)a.vocab + 2 * kPer - 2) / kPer / ranks + 1; };      // granules of a CTA, at most
-    // as many CTAs to a row as keep the SMs busy, a thousand elements each at least; more where the slice would be too long
+    // CTAs to a row: up to 96 in all, of two thousand elements each at least; up to 256, which share SMs, where each still has
+    // eight thousand; more where the slice would be too long.  Top-k and top-p / top-p alone, us, by CTAs a row:
+    //     1 x 4096      1: 8.3 / 11.2   2: 8.6 / 10.9   4: 8.9 / 12.4   8: 9.3 / 15.0
+    //    16 x 32000     2: 12.9 / 26.2  4: 11.1 / 19.6  8: 12.1 / 22.0
+    //    37 x 32000     1: 16.7 / 43.4  2: 13.2 / 27.3  4: 13.7 / 26.5  8: 21.6 / 39.3
+    //    64 x 32000     1: 16.8 / 45.4  2: 13.4 / 28.3  4: 14.7 / 27.8
+    //    32 x 128256    4: 17.8 / 51.8  8: 17.6 / 45.2
     int ranks = 1;
-    while (ranks < kMaxRanks && rows * ranks * 2 <= 296 && a.vocab / (ranks * 2) >= 1024) ranks *= 2;
+    while (ranks < kMaxRanks && a.vocab / (ranks * 2) >= 2048 &&
+           (rows * ranks * 2 <= 96 || rows * ranks * 2 <= 256 && a.vocab / (ranks * 2) >= 8192))
+        ranks *= 2;
     while (ranks < kMaxRanks && (slice(ranks) * 16 > (int64_t)kSampleSmem || slice(ranks) * kPer > kMaxSlice)) ranks *= 2;
     a.ranks = ranks;
     const size_t smem = (size_t)slice(ranks) * 16;
