@@ -5,15 +5,21 @@
 // tensor memory of its own; the scales are fp32, so no instruction applies them, and the epilogue warps take every finished
 // buffer into registers: acc += partial * (sx sw).  Two to four buffers keep the tensor core busy meanwhile.
 //
-// Two arrangements of the same pipeline:
-//   wide     the 128 lanes of tensor memory are rows of x, the columns 128 or 256 rows of the weight.  A thread owns a
-//            row of x and columns of one weight block: its scale is one number a block.
-//   swapped  (up to 64 rows of x) the lanes are weight rows, the columns 16, 32 or 64 rows of x, so that no tensor time
-//            and no bandwidth is spent on rows that are not there; a block's scales come as a row of shared memory.
+// Three arrangements of the same pipeline:
+//   swapped  (up to 64 rows of x) the lanes of tensor memory are 128 weight rows, the columns 16, 32 or 64 rows of x, so that no
+//            tensor time and no bandwidth is spent on rows that are not there; a block's scales come as a row of shared memory.
+//   wide     the lanes are 128 rows of x, the columns 128 rows of the weight.  A thread owns a row of x and columns of one
+//            weight block: its scale is one number a block.
+//   pairs    256 x 256 for two CTAs (further down).
 //
-//   warps 0 .. E-1   epilogue (E = 4, 8 from 64 columns on: 48 tokens, 14336 x 4096 with four warps 19.6 us, with eight 16.8 us)
+//   warps 0 .. E-1   epilogue (E = 4, 8 from 64 columns on)
 //   warp E           producer: per block of 128 K a box of both operands (128-byte swizzle) and the scales of x
 //   warp E + 1       tensor memory, MMA issue
+//
+// What bounds it.  One token, 128256 x 4096: HBM (79 us, 6.6 TB/s).  Few rows: a fixed 5 to 6 us (launch, set-up, first loads,
+// exchange) beside the weights' bytes; 48 x 14336 x 4096 also that 112 tiles keep 112 of 148 SMs busy (17.7 us, 3.4 TB/s).
+// Many rows: 4096 x 14336 x 4096 245 us, 1.96 PFLOP/s, in a burst and 284 us under the power cap; a block takes about 1060 cycles
+// of a pair for 512 of MMA, the rest is the way of a buffer from the MMA's end through the epilogue back to the issuer.
 //
 // Work split: an item is a tile of y.  A cluster of c CTAs (1, 2, 4 or 8) takes items in turn; its CTAs cut the blocks of K
 // in c runs, send their sums of 128 / c lanes to each CTA's shared memory and each CTA adds its lanes' in rank order: one launch,
@@ -458,8 +464,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             float acc[C::kPer];
 #pragma unroll
             for (int j = 0; j < C::kPer; ++j) acc[j] = 0.0f;
-            // Scales on their way kFar blocks ahead, in registers that take turns (moving one on would wait for it).  (They are not a stage's: a stage that stays until its scales have
-            // been read keeps the operands behind it waiting.)
+            // Scales on their way kFar blocks ahead, in registers that take turns: moving one on would wait for it.  They are not a
+            // stage's: one that stays until its scales have been read keeps the operands behind it waiting.
             constexpr int kFar = 4;
             const float *sx = a.sx + min(x0 + tl, a.m - 1) + k0 * a.ldsx, *sw_at = sw + k0;
             float sx_far[kFar], sw_far[kFar];
@@ -803,8 +809,19 @@ struct Fp8Choice {
     float cost = 1e30f;
     int cols = 0, cluster_log = 0, active = 0;
 };
-// An arrangement's cost in microseconds: rounds of items times blocks of K in a run.  Per block: what the weights of one SM
-// take from HBM, or the tensor core and the epilogue; per item: filling and draining the pipeline, an exchange.
+// An arrangement's cost in microseconds, up to what all have in common: rounds of items times blocks of K in a run.  Per block: what
+// the weights of one SM take from HBM, or the tensor core and the epilogue; per item: filling and draining the pipeline, an
+// exchange.  It picks, us on the device, * the choice:
+//     1 x 1024 x 4096     clusters of 1 9.9   2 8.3    4 6.7    8 6.3*
+//     1 x 4096 x 4096                1 10.2   2 9.5    4 8.8*   8 13.8
+//    16 x 4096 x 14336               1 28.5   2 19.1   4 15.5*  8 21.7
+//    48 x 14336 x 4096               1 17.6*  2 23.7   4 32.9
+//   100 x 4096 x 4096    wide        1 12.5   2 12.6   4 11.8*  pairs 20.9
+//   512 x 4096 x 4096                1 13.7*  2 22.6            pairs 21.9
+//   333 x 1000 x 1500                1 9.4    2 8.9    4 8.9*   pairs 15.5
+//   300 x 14337 x 4096               1 42.7*  2 52.4            pairs 51.1
+//  1024 x 4096 x 4096                1 24.0   2 41.7            pairs 22.5*
+//  2048 x 4096 x 4096                1 43.8   2 74.6            pairs 40.8*
 template <int kCols, bool kSwap, bool kOwn>
 int consider(const Fp8Args& a, Fp8Choice& best) {
     static ActiveClusters active;
@@ -830,7 +847,7 @@ int consider_pair(const Fp8Args& a, Fp8Choice& best) {
     if (const int rc = active_clusters(active, reinterpret_cast<const void*>(fp8_pair_kernel), kPairThreads, kPairBytes, clusters)) return rc;
     if (clusters[1] < 1) return MIXFP4_OK;
     const int64_t items = (int64_t)((a.m + 255) / 256) * ((a.n + 255) / 256), rounds = (items + clusters[1] - 1) / clusters[1];
-    const float cost = (float)rounds * (0.36f * (float)a.blocks + 1.5f);
+    const float cost = (float)rounds * (0.36f * (float)a.blocks + (a.y_vec ? 1.5f : 5.5f));     // stores through the patches show
     if (cost < best.cost) best = Fp8Choice{cost, 256, 1, clusters[1]};
     return MIXFP4_OK;
 }
