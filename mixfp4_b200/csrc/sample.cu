@@ -22,7 +22,8 @@
 // one row of 128256 logits with top-k and top-p; this takes 13).  Large batches: the fp64 operations of the weights, in a pass
 // with all of them 14 us for the 64 K elements of an SM, and the histogram's additions in shared memory.
 // Measured and not kept: lists of a warp's few elements of interest, sorting the candidates, sums of what a top-p cannot reach
-// beside the histogram (each more code than it saved time: 64 mixed rows 61 us, so 69 to 79).
+// beside the histogram, a first histogram over the topmost bf16 keys instead of equal widths (each more code than it saved time:
+// 64 mixed rows 61 to 65 us, so 69 to 79).
 
 #include <float.h>
 
