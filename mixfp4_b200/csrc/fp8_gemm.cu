@@ -203,12 +203,16 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, cons
     return true;
 }
 
-__device__ __forceinline__ void store_one(const Fp8Args& a, int64_t row, int64_t col, float v) {
-    const int64_t at = row * a.ldy + col;
-    if (a.out_dtype == MIXFP4_F32) static_cast<float*>(a.y)[at] = v;
-    else if (a.out_dtype == MIXFP4_BF16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(a.y)[at] = __float2half_rn(v);
+// f(y) with the output's type.  Around whole loops: a kernel of few rows runs its stores once, and what it fetches of its code on the
+// way counts.
+template <typename F>
+__device__ __forceinline__ void with_output(const Fp8Args& a, F&& f) {
+    if (a.out_dtype == MIXFP4_BF16) f(static_cast<__nv_bfloat16*>(a.y));
+    else if (a.out_dtype == MIXFP4_F32) f(static_cast<float*>(a.y));
+    else f(static_cast<__half*>(a.y));
 }
+template <typename T>
+__device__ __forceinline__ void put(T* p, float v) { *p = Elem<T>::round(v); }
 // 32 aligned bytes, a whole sector of the L2.
 __device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
@@ -230,9 +234,11 @@ __device__ __forceinline__ void store_run(const Fp8Args& a, int64_t row0, int64_
             __syncwarp();
             const int j = lane % kPatchCols;
             if (col + c + j < a.n) {
+                with_output(a, [&](auto* y) {
 #pragma unroll 8
-                for (int i = lane / kPatchCols; i < 32; i += 32 / kPatchCols)
-                    if (row0 + i < a.m) store_one(a, row0 + i, col + c + j, patch[i * kPatchPitch + j]);
+                    for (int i = lane / kPatchCols; i < 32; i += 32 / kPatchCols)
+                        if (row0 + i < a.m) put(y + (row0 + i) * a.ldy + col + c + j, patch[i * kPatchPitch + j]);
+                });
             }
             __syncwarp();
         }
@@ -506,11 +512,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             if (!ok) break;
             if (a.cluster == 1) {
                 if constexpr (kSwap) {
-                    if (w0 + tl < a.n) {
+                    if (w0 + tl < a.n)
+                        with_output(a, [&](auto* y) {
+                            const int row = x0 + half * C::kPer;
+                            y += row * a.ldy + w0 + tl;
 #pragma unroll
-                        for (int j = 0; j < C::kPer; ++j)
-                            if (x0 + half * C::kPer + j < a.m) store_one(a, x0 + half * C::kPer + j, w0 + tl, acc[j]);
-                    }
+                            for (int j = 0; j < C::kPer; ++j, y += a.ldy)
+                                if (row + j < a.m) put(y, acc[j]);
+                        });
                 } else {
                     store_run<C::kPer>(a, x0 + quad * 32, w0 + half * C::kPer, acc, reinterpret_cast<float*>(gen + L.patches + warp * kPatchBytes));
                 }
@@ -534,21 +543,24 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             if (!ok) break;
             xph ^= 1;
             const int groups = kCols / 4;                               // four columns of a lane at a time
-            for (int i = threadIdx.x; i < share * groups; i += C::kEpi * 32) {
-                const int l = kSwap ? i % share : i / groups, c = (kSwap ? i / share : i % groups) * 4;
-                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int r = 0; r < a.cluster; ++r) {
-                    const float4 v = lds_f32x4(xbuf + r * slot + c / 4 * pitch + l * 16u);
-                    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-                }
-                const float e[4] = {sum.x, sum.y, sum.z, sum.w};
-                const int tile_lane = rank * share + l;
+            with_output(a, [&](auto* y) {
+#pragma unroll 1
+                for (int i = threadIdx.x; i < share * groups; i += C::kEpi * 32) {
+                    const int l = kSwap ? i % share : i / groups, c = (kSwap ? i / share : i % groups) * 4;
+                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+                    for (int r = 0; r < a.cluster; ++r) {
+                        const float4 v = lds_f32x4(xbuf + r * slot + c / 4 * pitch + l * 16u);
+                        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+                    }
+                    const float e[4] = {sum.x, sum.y, sum.z, sum.w};
+                    const int row = x0 + (kSwap ? c : rank * share + l), col = w0 + (kSwap ? rank * share + l : c);
+                    auto* p = y + row * a.ldy + col;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int64_t row = kSwap ? x0 + c + j : x0 + tile_lane, col = kSwap ? w0 + tile_lane : w0 + c + j;
-                    if (row < a.m && col < a.n) store_one(a, row, col, e[j]);
+                    for (int j = 0; j < 4; ++j, p += kSwap ? a.ldy : 1)
+                        if (row + (kSwap ? j : 0) < a.m && col + (kSwap ? 0 : j) < a.n) put(p, e[j]);
                 }
-            }
+            });
             __syncwarp();
             if (lane < a.cluster) arrive_peer(peer_addr(sums_out, lane));
         }
