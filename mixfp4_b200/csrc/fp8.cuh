@@ -10,8 +10,8 @@ constexpr int kFp8Block = 128;
 __host__ __device__ inline int64_t fp8_scale_rows(int64_t m) { return (m + 127) / 128 * 128; }
 
 // Whether a product quantizes a dense x itself, in every CTA: up to 256 row blocks and 48 blocks of K (what shared memory holds
-// of it beside the weights' ring).  Itself / by a kernel ahead of it, on the device: 1 x 4096 x 4096 8.7 / 10.6 us, 4 rows
-// 9.3 / 10.6, 8 rows (256 blocks) 10.0 / 10.7, 16 rows (512) 11.3 / 10.7, 32 x 4096 x 1024 8.7 / 8.2; and the host has
+// of it beside the weights' ring).  Itself / by a kernel ahead of it, on the device: 1 x 4096 x 4096 8.3 / 10.1 us, 4 rows
+// 8.8 / 10.1, 8 rows (256 blocks) 9.4 / 10.0, 16 rows (512) 10.9 / 10.0, 32 x 4096 x 1024 (256) 8.0 / 7.3; and the host has
 // one launch and no workspace for it.
 inline bool fp8_quantizes_itself(int64_t m, int64_t k) {
     const int64_t blocks = (k + kFp8Block - 1) / kFp8Block;

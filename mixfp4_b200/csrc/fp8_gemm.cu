@@ -17,7 +17,7 @@
 //   warp E + 1       tensor memory, MMA issue
 //
 // What bounds it.  One token, 128256 x 4096: HBM (79 us, 6.6 TB/s).  Few rows: a fixed 5 to 6 us (launch, set-up, first loads,
-// exchange) beside the weights' bytes; 48 x 14336 x 4096 also that 112 tiles keep 112 of 148 SMs busy (17.7 us, 3.4 TB/s).
+// exchange) beside the weights' bytes; 48 x 14336 x 4096 also that 112 tiles keep 112 of 148 SMs busy (15.7 us, 3.8 TB/s).
 // Many rows: 4096 x 14336 x 4096 245 us, 1.96 PFLOP/s, in a burst and 284 us under the power cap; a block takes about 1060 cycles
 // of a pair for 512 of MMA, the rest is the way of a buffer from the MMA's end through the epilogue back to the issuer.
 //
@@ -219,7 +219,7 @@ __device__ __forceinline__ void st_sector(void* p, const uint32_t (&w)[8]) {
                  ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 // kN consecutive columns of this lane's row, row0 + lane, by a whole warp.  A sector at a time where rows of y are whole sectors;
-// otherwise through the warp's patch (4096 x 4099 x 4096 bf16: 98 us, 4096 x 1000 x 4096: 27 us; each thread storing its row's
+// otherwise through the warp's patch (4096 x 4099 x 4096 bf16: 95 us, 4096 x 1000 x 4096: 26 us; each thread storing its row's
 // columns one by one, 32 sectors an instruction: 231 us and 61 us).
 template <int kN>
 __device__ __forceinline__ void store_run(const Fp8Args& a, int64_t row0, int64_t col, const float (&v)[kN], float* patch) {
@@ -469,27 +469,33 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             float acc[C::kPer];
 #pragma unroll
             for (int j = 0; j < C::kPer; ++j) acc[j] = 0.0f;
-            // Scales on their way kFar blocks ahead, in registers that take turns: moving one on would wait for it.  They are not a
-            // stage's: one that stays until its scales have been read keeps the operands behind it waiting.
-            constexpr int kFar = 4;
+            // Swapped: the weight's scales of 32 blocks, a lane each.  Wide: both scales on their way kFar blocks ahead, in registers
+            // that take turns (moving one on would wait for it); they are not a stage's, since one that stays until its scales have
+            // been read keeps the operands behind it waiting.  No more copies of the loop's body than that: its code is fetched once
+            // for few blocks (48 x 14336 x 4096 with four copies 15.9 us, with one 15.7; 1 x 14336 x 4096 12.7 and 12.4).
+            constexpr int kFar = kSwap ? 1 : 2;
             const float *sx = a.sx + min(x0 + tl, a.m - 1) + k0 * a.ldsx, *sw_at = sw + k0;
-            float sx_far[kFar], sw_far[kFar];
+            float sx_far[kFar], sw_far[kFar], sw_lanes = 0.0f;
             auto fetch_scales = [&](int i, bool more) {
-                if (more) {
-                    sw_far[i] = __ldg(sw_at);
-                    if constexpr (!kSwap) sx_far[i] = __ldcg(sx);
+                if constexpr (!kSwap) {
+                    if (more) {
+                        sw_far[i] = __ldg(sw_at);
+                        sx_far[i] = __ldcg(sx);
+                    }
+                    ++sw_at;
+                    sx += a.ldsx;
                 }
-                ++sw_at;
-                if constexpr (!kSwap) sx += a.ldsx;
             };
 #pragma unroll
             for (int i = 0; i < kFar; ++i) fetch_scales(i, k0 + i < k1);
-            for (int kb4 = k0; kb4 < k1 && ok; kb4 += kFar)
+            for (int kb0 = k0; kb0 < k1 && ok; kb0 += kFar)
 #pragma unroll
             for (int turn = 0; turn < kFar; ++turn) {
-                const int kb = kb4 + turn;
+                const int kb = kb0 + turn;
                 if (kb >= k1) break;
-                const float sw_now = sw_far[turn], row_scale = kSwap ? 0.0f : sx_far[turn] * sw_now;
+                if (kSwap && (kb - k0) % 32 == 0) sw_lanes = kb + lane < k1 ? __ldg(sw + kb + lane) : 0.0f;
+                const float sw_now = kSwap ? __shfl_sync(0xffffffffu, sw_lanes, (kb - k0) % 32) : sw_far[turn];
+                const float row_scale = kSwap ? 0.0f : sx_far[turn] * sw_now;
                 fetch_scales(turn, kb + kFar < k1);
                 ok = __all_sync(0xffffffffu, mbar_wait(acc_full(b), bph, ctx, 24) && (!kRingScales || mbar_wait(full(s), ph, ctx, 25)));
                 if (!ok) break;
@@ -826,16 +832,16 @@ struct Fp8Choice {
 // An arrangement's cost in microseconds, up to what all have in common: rounds of items times blocks of K in a run.  Per block: what
 // the weights of one SM take from HBM, or the tensor core and the epilogue; per item: filling and draining the pipeline, an
 // exchange.  It picks, us on the device, * the choice:
-//     1 x 1024 x 4096     clusters of 1 9.9   2 8.3    4 6.7    8 6.3*
-//     1 x 4096 x 4096                1 10.2   2 9.5    4 8.8*   8 13.8
-//    16 x 4096 x 14336               1 28.5   2 19.1   4 15.5*  8 21.7
-//    48 x 14336 x 4096               1 17.6*  2 23.7   4 32.9
-//   100 x 4096 x 4096    wide        1 12.5   2 12.6   4 11.8*  pairs 20.9
-//   512 x 4096 x 4096                1 13.7*  2 22.6            pairs 21.9
-//   333 x 1000 x 1500                1 9.4    2 8.9    4 8.9*   pairs 15.5
-//   300 x 14337 x 4096               1 42.7*  2 52.4            pairs 51.1
-//  1024 x 4096 x 4096                1 24.0   2 41.7            pairs 22.5*
-//  2048 x 4096 x 4096                1 43.8   2 74.6            pairs 40.8*
+//     1 x 1024 x 4096     clusters of 1 9.4   2 7.7    4 6.1    8 5.7*
+//     1 x 4096 x 4096                1 9.6    2 8.9    4 8.1*   8 12.8
+//    16 x 4096 x 14336               1 27.2   2 17.8   4 14.9*  8 21.2
+//    48 x 14336 x 4096               1 16.0*  2 21.4   4 28.2
+//   100 x 4096 x 4096    wide        1 12.6   2 11.4   4 10.3*  pairs 20.9
+//   512 x 4096 x 4096                1 13.8*  2 21.0            pairs 21.7
+//   333 x 1000 x 1500                1 9.3    2 7.9    4 7.8*   pairs 14.8
+//   300 x 14337 x 4096               1 42.2*  2 48.9            pairs 49.7
+//  1024 x 4096 x 4096                1 24.0   2 40.7            pairs 22.3*
+//  2048 x 4096 x 4096                1 43.8   2 66.5            pairs 40.4*
 template <int kCols, bool kSwap, bool kOwn>
 int consider(const Fp8Args& a, Fp8Choice& best) {
     static ActiveClusters active;
