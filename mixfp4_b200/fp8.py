@@ -11,6 +11,7 @@ counterpart of this format in it.  Inputs that are not finite make their block's
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 
@@ -205,6 +206,12 @@ def dequantize_fp8(q: FP8Weight | FP8Activations, dtype: torch.dtype = torch.bfl
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(m: int, k: int) -> int:
+    """The library's answer, a function of the sizes alone: half a microsecond less than asking again."""
+    return nat.lib().mixfp4_fp8_workspace_bytes(m, k)
+
+
 def fp8_linear(x: torch.Tensor | FP8Activations, weight: FP8Weight, *, bias: torch.Tensor | None = None,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y = x @ W^T (+ bias) on block-scaled FP8 operands.  x: a dense tensor [..., K] (bf16, f16 or fp32), quantized within
@@ -235,7 +242,7 @@ def fp8_linear(x: torch.Tensor | FP8Activations, weight: FP8Weight, *, bias: tor
                                          _status_word(device).data_ptr(), stream)
                 nat.check("mixfp4_fp8_gemm", st)
             else:
-                nbytes = lib.mixfp4_fp8_workspace_bytes(m, k)
+                nbytes = _workspace_bytes(m, k)
                 work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None      # a captured graph's own
                 st = lib.mixfp4_fp8_linear(x2.data_ptr(), nat.DTYPE_CODE[x2.dtype], m, x2.stride(0), codes.data_ptr(),
                                            codes.stride(0), weight.scales.data_ptr(), n, k, y.data_ptr(), out_code, n,

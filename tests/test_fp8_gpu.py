@@ -338,3 +338,13 @@ def test_rows_of_y_at_any_offset_and_stride(m, n, dtype):
         rows = held[offset: offset + m * ldy].view(m, ldy)
         assert torch.equal(rows[:, :n], want), (offset, ldy)
         assert (held[:offset] == 7).all() and (rows[:, n:] == 7).all() and (held[offset + m * ldy:] == 7).all()
+
+
+def test_outputs_past_2_31_elements():
+    m, n, k = 17000, 128256, 128                             # 2.18e9 elements
+    x, w = _data(m, k, torch.bfloat16, 61, spread=False), _data(n, k, torch.bfloat16, 62, spread=False)
+    weight, q = mx.quantize_fp8_weight(w), mx.quantize_fp8_activations(x)
+    y = mx.fp8_linear(q, weight)
+    a, b = _expand(q.codes, q.scales, 1), _expand(weight.codes, weight.scales, 128)
+    for rows, cols in ((slice(0, 3), slice(0, n)), (slice(m - 3, m), slice(0, n)), (slice(0, m), slice(n - 5, n))):
+        _check_product(y[rows, cols], a[rows], b[cols], torch.bfloat16)
