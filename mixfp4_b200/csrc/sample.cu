@@ -489,30 +489,27 @@ struct Sampler {
                 for (int c = c0 + lane; c < c1; c += 32) {
                     float x[4];
                     get(c, x);
-                    uint32_t at[4];
-                    bool hit[4];
+                    if (!(x[0] >= from || x[1] >= from || x[2] >= from || x[3] >= from)) continue;
+                    if (level == 0) {                    // most of them count: four at once
+                        u64 w[4] = {};
+                        if (by_mass) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        at[j] = linear(x[j]);
-                        hit[j] = x[j] >= from && (level == 0 || at[j] == bin);
-                    }
-                    if (!(hit[0] || hit[1] || hit[2] || hit[3])) continue;
-                    if (level > 0) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t key = Row<T>::key(x[j]);
-                            hit[j] = hit[j] && key >= lo && key <= hi;
-                            at[j] = (hi - key) >> shift;
+                            for (int j = 0; j < 4; ++j) w[j] = weight(fmaxf(x[j], floor_x));
                         }
-                    }
-                    u64 w[4] = {};
-                    if (by_mass) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) w[j] = weight(fmaxf(x[j], floor_x));
+                        for (int j = 0; j < 4; ++j)
+                            if (x[j] >= from) put(linear(x[j]), !by_mass, w[j]);
+                        continue;
                     }
+                    uint32_t hits = 0;                   // few do: one at a time
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (hit[j]) put(at[j], !by_mass || level > 0, w[j]);
+                    for (int j = 0; j < 4; ++j) hits |= x[j] >= from && linear(x[j]) == bin ? 1u << j : 0u;
+#pragma unroll 1
+                    for (; hits; hits &= hits - 1) {
+                        const float v = hits & 1 ? x[0] : hits & 2 ? x[1] : hits & 4 ? x[2] : x[3];
+                        const uint32_t key = Row<T>::key(v);
+                        if (key >= lo && key <= hi) put((hi - key) >> shift, true, by_mass ? weight(v) : 0);
+                    }
                 }
                 goal = find(by_mass, before, goal, p, out);
                 const uint32_t b = s.found_bin;
