@@ -16,17 +16,17 @@ namespace {
 // A group of eight lanes per row and block.  scales: [block][lds], a row's scales a column of it, so that the product reads
 // the scales of neighbouring rows together.
 template <typename T>
-__global__ void __launch_bounds__(256) fp8_rows_kernel(const T* x, int64_t m, int64_t k, int64_t ldx, bool vec,
+__global__ void __launch_bounds__(256) fp8_rows_kernel(const T* x, uint32_t total, uint32_t blocks, int64_t k, int64_t ldx, bool vec,
                                                        uint8_t* codes, int64_t ldq, float* scales, int64_t lds) {
     asm volatile("griddepcontrol.wait;" ::: "memory");                       // x may be the kernel before's output
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int64_t blocks = (k + kFp8Block - 1) / kFp8Block, total = m * blocks;
     const int sub = threadIdx.x % kLanesPerRow;
-    const int64_t stride = (int64_t)gridDim.x * (blockDim.x / kLanesPerRow);
-    for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / kLanesPerRow) + threadIdx.x / kLanesPerRow;; i += stride) {
+    const uint32_t stride = gridDim.x * (256 / kLanesPerRow);
+    for (uint32_t i = blockIdx.x * (256 / kLanesPerRow) + threadIdx.x / kLanesPerRow;; i += stride) {
         const bool in = i < total;
         if (!__any_sync(0xffffffffu, in)) break;
-        const int64_t row = in ? i / blocks : 0, b = in ? i - row * blocks : 0;
+        const uint32_t at = in ? i / blocks : 0;
+        const int64_t row = at, b = in ? i - at * blocks : 0;
         const int64_t c = b * kFp8Block + sub * kLaneElems;
         Raw<T> v;
         load16(x + row * ldx, c, in ? k : 0, vec, v);
@@ -112,6 +112,7 @@ int fp8_check_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx, 
     if (dtype != MIXFP4_BF16 && dtype != MIXFP4_F16 && dtype != MIXFP4_F32) return MIXFP4_E_DTYPE;
     if (m <= 0 || k <= 0 || m > kMaxSide || k > kMaxSide - 128 || ldx < k || ldq < padded_k(k) || lds < fp8_scale_rows(m))
         return MIXFP4_E_SHAPE;
+    if (m * ((k + kFp8Block - 1) / kFp8Block) > kMaxSide) return MIXFP4_E_SHAPE;      // 2^38 elements
     if (!aligned(x, fp8_elem_bytes(dtype)) || !aligned(codes, 16) || ldq % 16 != 0 || !aligned(scales, 16) || lds % 4 != 0)
         return MIXFP4_E_ALIGN;
     return MIXFP4_OK;
@@ -122,7 +123,7 @@ int fp8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t ld
     return by_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
         const bool vec = aligned(x, 16) && ldx * (int64_t)sizeof(T) % 16 == 0;
-        const int64_t groups = m * ((k + kFp8Block - 1) / kFp8Block), per_cta = 256 / kLanesPerRow;
+        const int64_t blocks = (k + kFp8Block - 1) / kFp8Block, groups = m * blocks, per_cta = 256 / kLanesPerRow;
         const int64_t ctas = (groups + per_cta - 1) / per_cta;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(ctas < 148 * 64 ? ctas : 148 * 64));
@@ -133,7 +134,7 @@ int fp8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t ld
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        MIXFP4_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fp8_rows_kernel<T>, static_cast<const T*>(x), m, k, ldx, vec, codes, ldq,
+        MIXFP4_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fp8_rows_kernel<T>, static_cast<const T*>(x), (uint32_t)groups, (uint32_t)blocks, k, ldx, vec, codes, ldq,
                                              scales, lds));
         return check_launch("fp8_rows_kernel");
     });
