@@ -13,7 +13,8 @@
 namespace mixfp4 {
 namespace {
 
-// A group of eight lanes per row and block.  scales: [block][lds], a row's scales a column of it, so that the product reads
+// A group of eight lanes per row and block (4096 x 4096 bf16: 11.4 us, 4.4 TB/s, bound by instruction issue as much as by loads; two
+// blocks a group with their loads ahead 12.1 to 16.4, four 14.3; with 64-bit indices 12.1).  scales: [block][lds], a row's scales a column of it, so that the product reads
 // the scales of neighbouring rows together.
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_rows_kernel(const T* x, uint32_t total, uint32_t blocks, int64_t k, int64_t ldx, bool vec,
