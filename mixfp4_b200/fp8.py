@@ -149,15 +149,16 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
     nat.require_cuda(x, what)
     if x.dtype not in nat.DTYPE_CODE:
         raise TypeError(f"{what} must be bfloat16, float16 or float32")
-    if x.ndim == 0 or x.shape[-1] == 0:
+    shape = x.shape
+    if len(shape) == 0 or shape[-1] == 0:
         raise ValueError(f"{what} must have at least one column")
-    x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
-    if x2.stride(0) >= x2.shape[1] and x2.stride(1) == 1:
+    x2 = x if len(shape) == 2 else x.reshape(-1, shape[-1])
+    ld, step = x2.stride()
+    if ld >= shape[-1] and step == 1:
         return x2
-    if x2.stride(1) != 1 or x2.stride(0) < x2.shape[1]:
-        x2 = x2.reshape(1, -1) if x2.shape[0] == 1 and x2.stride(1) == 1 else x2.contiguous()
-        if x2.stride(0) < x2.shape[1]:                   # a single row, whose stride can be any number
-            x2 = x2.as_strided(x2.shape, (x2.shape[1], 1))
+    x2 = x2.reshape(1, -1) if x2.shape[0] == 1 and step == 1 else x2.contiguous()
+    if x2.stride(0) < shape[-1]:                         # a single row, whose stride can be any number
+        x2 = x2.as_strided(x2.shape, (shape[-1], 1))
     return x2
 
 

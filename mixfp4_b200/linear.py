@@ -22,7 +22,7 @@ GEMV_MAX_M = 16
 GROUPED_MAX_M = 64       # rows of x that mixfp4_gemm_grouped takes
 SMALL_MAX_M = 128        # rows that run without split-K partial sums on the kernel and stream layouts
 _workspaces: dict[tuple, torch.Tensor] = {}
-_status_words: dict[str, torch.Tensor] = {}
+_status_words: dict[torch.device, torch.Tensor] = {}
 
 
 def _workspace(device, nbytes: int) -> torch.Tensor | None:
@@ -37,10 +37,10 @@ def _workspace(device, nbytes: int) -> torch.Tensor | None:
 
 
 def _status_word(device) -> torch.Tensor:
-    key = str(device)
-    if key not in _status_words:
-        _status_words[key] = torch.zeros(1, dtype=torch.int32, device=device)
-    return _status_words[key]
+    word = _status_words.get(device)
+    if word is None:
+        word = _status_words[device] = torch.zeros(1, dtype=torch.int32, device=device)
+    return word
 
 
 def gemm_status(device=None) -> int:
