@@ -334,9 +334,9 @@ struct Sampler {
         if (a.logprob) a.logprob[r] = greedy ? 0.0f : (float)((x == largest ? 0.0 : ((double)x - top) * inv_t) - log_of(total));
     }
 
-    // At most kFew candidates, the elements of the linear bins up to `bin`: rank 0 takes them all, two threads to each, and
+    // At most kFew candidates, the elements from `from` on in the linear bins up to `bin`, as they were counted: rank 0 takes them all, two threads to each, and
     // adds up what goes before it, by value and then, of the kept ones, by index.
-    __device__ void choose_from_few(int64_t r, uint32_t bin, uint32_t k, double p, u64 lowest, double u) {
+    __device__ void choose_from_few(int64_t r, float from, uint32_t bin, uint32_t k, double p, u64 lowest, double u) {
         const uint32_t count_at = of_rank(shared_addr(&s.few_count), 0), few_at = of_rank(shared_addr(s.few), 0);
 #pragma unroll 1
         for (int c = c0 + lane; c < c1; c += 32) {
@@ -344,7 +344,7 @@ struct Sampler {
             get(c, x);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (x[j] < floor_x || linear(x[j]) > bin) continue;
+                if (!(x[j] >= from) || linear(x[j]) > bin) continue;
                 const uint32_t at = add_rank32(count_at, 1), index = (uint32_t)(c * 4 + j - skew);
                 if (at < kFew) st_rank64(few_at + at * 8, (u64)Row<T>::key(x[j]) << 32 | (uint32_t)~index);
             }
@@ -517,7 +517,7 @@ struct Sampler {
                 const uint32_t size = s.found_size;
                 if (b == (uint32_t)kBins) break;         // fewer than k have a weight: all of them stay
                 if (level == 0) {
-                    if (!by_mass && before + size <= kFew) return choose_from_few(r, b, (uint32_t)k, p, lowest, u);
+                    if (!by_mass && before + size <= kFew) return choose_from_few(r, from, b, (uint32_t)k, p, lowest, u);
                     // keys that the bin can hold: its edges, moved out by more than rounding moved them
                     bin = b;
                     const float width = 1.0f / bin_scale;

@@ -231,3 +231,13 @@ def test_values_and_temperatures_near_the_ends_of_fp32(temperature):
         u = torch.rand(4, generator=g).cuda()
         for settings in (dict(), dict(top_k=700), dict(top_p=0.6), dict(top_k=2000, top_p=0.99)):
             _check(x, u, temperature=temperature, **settings)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_logits_closer_together_than_a_bin(dtype):
+    """All of a row within a bin or two: a top-k's candidates are those that were counted, not all that share their bin."""
+    for rows, vocab, scale in ((20, 1500, 0.01), (6, 9000, 0.003), (3, 40003, 0.02)):
+        for k in (1, 2, 20, 200):
+            x, u = _logits(rows, vocab, dtype, 71 + k, scale)
+            for settings in (dict(temperature=1.5), dict(top_p=0.5), dict(temperature=20.0, min_p=0.9)):
+                _check(x, u, top_k=k, **settings)
