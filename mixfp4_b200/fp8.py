@@ -73,6 +73,14 @@ class FP8Weight:
         self.n, self.k = self.codes.shape
 
     @classmethod
+    def _made(cls, codes, scales) -> "FP8Weight":
+        """Parts that this module made itself: nothing to check."""
+        w = object.__new__(cls)
+        w.codes, w.scales = codes, scales
+        w.n, w.k = codes.shape
+        return w
+
+    @classmethod
     def from_tensors(cls, codes: torch.Tensor, scales: torch.Tensor) -> "FP8Weight":
         """Codes (float8_e4m3fn or their bytes) and scales of a checkpoint; copied only where their rows are not aligned."""
         codes = _check_parts(codes, scales, FP8_BLOCK)
@@ -141,7 +149,7 @@ class FP8Activations:
 def _scale_room(m: int, k: int, device) -> torch.Tensor:
     room = _blocks(m) * FP8_BLOCK
     held = torch.empty_strided((room, _blocks(k)), (1, room), dtype=torch.float32, device=device)
-    return held if m == room else held[:m]
+    return held if m == room else held.narrow(0, 0, m)
 
 
 def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
@@ -166,15 +174,17 @@ def quantize_fp8_weight(w: torch.Tensor) -> FP8Weight:
     """A dense [n, k] weight (bf16, f16 or fp32, on the GPU) to codes and a scale for every 128 x 128 tile, in one pass."""
     if w.ndim != 2 or 0 in w.shape:
         raise ValueError("the weight must be a matrix with at least one row and column")
-    w = _rows(w.detach(), "the weight")
-    n, k = w.shape
-    codes = torch.empty((n, _blocks(k) * FP8_BLOCK), dtype=torch.float8_e4m3fn, device=w.device)
-    scales = torch.empty((_blocks(n), _blocks(k)), dtype=torch.float32, device=w.device)
-    with nat.on_device(w.device):
-        st = nat.lib().mixfp4_fp8_quantize_tiles(w.data_ptr(), nat.DTYPE_CODE[w.dtype], n, k, w.stride(0), codes.data_ptr(),
-                                                 codes.stride(0), scales.data_ptr(), nat.stream_ptr(w.device))
+    w = _rows(w, "the weight")
+    (n, k), device = w.shape, w.device
+    blocks = _blocks(k)
+    ld = blocks * FP8_BLOCK
+    codes = torch.empty_strided((n, ld), (ld, 1), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty_strided((_blocks(n), blocks), (blocks, 1), dtype=torch.float32, device=device)
+    with nat.on_device(device):
+        st = nat.lib().mixfp4_fp8_quantize_tiles(w.data_ptr(), nat.DTYPE_CODE[w.dtype], n, k, w.stride(0), codes.data_ptr(), ld,
+                                                 scales.data_ptr(), nat.stream_ptr(device))
     nat.check("mixfp4_fp8_quantize_tiles", st)
-    return FP8Weight(codes if codes.shape[1] == k else codes[:, :k], scales)
+    return FP8Weight._made(codes if ld == k else codes.narrow(1, 0, k), scales)
 
 
 def quantize_fp8_activations(x: torch.Tensor) -> FP8Activations:
@@ -189,7 +199,7 @@ def quantize_fp8_activations(x: torch.Tensor) -> FP8Activations:
             st = nat.lib().mixfp4_fp8_quantize_rows(x2.data_ptr(), nat.DTYPE_CODE[x.dtype], m, k, x2.stride(0), codes.data_ptr(), ld,
                                                     scales.data_ptr(), _blocks(m) * FP8_BLOCK, nat.stream_ptr(device))
         nat.check("mixfp4_fp8_quantize_rows", st)
-    return FP8Activations._made(codes if ld == k else codes[:, :k], scales, x.shape, x.dtype)
+    return FP8Activations._made(codes if ld == k else codes.narrow(1, 0, k), scales, x.shape, x.dtype)
 
 
 def dequantize_fp8(q: FP8Weight | FP8Activations, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
