@@ -18,7 +18,7 @@
 //
 // What bounds it.  One token, 128256 x 4096: HBM (79 us, 6.6 TB/s).  Few rows: a fixed 5 to 6 us (launch, set-up, first loads,
 // exchange) beside the weights' bytes; 48 x 14336 x 4096 also that 112 tiles keep 112 of 148 SMs busy (15.7 us, 3.8 TB/s).
-// Many rows: 4096 x 14336 x 4096 245 us, 1.96 PFLOP/s, in a burst and 284 us under the power cap; a block takes about 1060 cycles
+// Many rows: 4096 x 14336 x 4096 242 us, 1.99 PFLOP/s, in a burst and 284 us under the power cap; a block takes about 1060 cycles
 // of a pair for 512 of MMA, the rest is the way of a buffer from the MMA's end through the epilogue back to the issuer.
 //
 // Work split: an item is a tile of y.  A cluster of c CTAs (1, 2, 4 or 8) takes items in turn; its CTAs cut the blocks of K
@@ -588,9 +588,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 
 // ------------------------------------------------------------------- CTA pairs
 // A tile of 256 x 256 for two CTAs: 128 rows of x and half of the weight rows each, one tcgen05.mma.cta_group::2 over both (M
-// 256, N 256).  What bounds a single CTA's 128 x 256 is the way from the L2 into an SM (64 bytes a cycle): 48 KB a block, 760
-// cycles for 512 cycles of MMA; the pair's CTAs fetch 32 KB each.  The even CTA (the leader) issues; its full barriers count
-// both CTAs' bytes, its commits release stages and report buffers in both, its acc_empty counts both CTAs' epilogue warps.
+// 256, N 256).  A CTA fetches 32 KB a block for 128 x 256 products, where one alone would fetch 48 (4096 x 14336 x 4096: pairs 242 us,
+// 128 x 256 on single CTAs 325, 128 x 128 273; the pairs' own pace without their epilogue's reads 197).  The even CTA (the leader)
+// issues; its full barriers count both CTAs' bytes, its commits release stages and report buffers in both, its acc_empty counts
+// both CTAs' epilogue warps.
 constexpr uint32_t kLeaderMask = 0xFEFFFFFFu;        // clears the CTA-rank bit of a shared::cluster address
 constexpr int kPairEpi = 8, kPairThreads = (kPairEpi + 4) * 32, kPairStages = 6, kPairBufs = 2;
 constexpr uint32_t kPairHalf = 128 * 128, kPairStage = 2 * kPairHalf, kPairPatches = kPairStages * kPairStage, kPairBars = kPairPatches + kPairEpi * kPatchBytes;

@@ -147,9 +147,9 @@ class FP8Activations:
 
 
 def _scale_room(m: int, k: int, device) -> torch.Tensor:
-    room = _blocks(m) * FP8_BLOCK
-    held = torch.empty_strided((room, _blocks(k)), (1, room), dtype=torch.float32, device=device)
-    return held if m == room else held.narrow(0, 0, m)
+    room, blocks = _blocks(m) * FP8_BLOCK, _blocks(k)
+    held = torch.empty_strided((room, blocks), (1, room), dtype=torch.float32, device=device)
+    return held if m == room else held.as_strided((m, blocks), (1, room))      # a microsecond less than a slice
 
 
 def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
@@ -184,7 +184,7 @@ def quantize_fp8_weight(w: torch.Tensor) -> FP8Weight:
         st = nat.lib().mixfp4_fp8_quantize_tiles(w.data_ptr(), nat.DTYPE_CODE[w.dtype], n, k, w.stride(0), codes.data_ptr(), ld,
                                                  scales.data_ptr(), nat.stream_ptr(device))
     nat.check("mixfp4_fp8_quantize_tiles", st)
-    return FP8Weight._made(codes if ld == k else codes.narrow(1, 0, k), scales)
+    return FP8Weight._made(codes if ld == k else codes.as_strided((n, k), (ld, 1)), scales)
 
 
 def quantize_fp8_activations(x: torch.Tensor) -> FP8Activations:
@@ -199,7 +199,7 @@ def quantize_fp8_activations(x: torch.Tensor) -> FP8Activations:
             st = nat.lib().mixfp4_fp8_quantize_rows(x2.data_ptr(), nat.DTYPE_CODE[x.dtype], m, k, x2.stride(0), codes.data_ptr(), ld,
                                                     scales.data_ptr(), _blocks(m) * FP8_BLOCK, nat.stream_ptr(device))
         nat.check("mixfp4_fp8_quantize_rows", st)
-    return FP8Activations._made(codes if ld == k else codes.narrow(1, 0, k), scales, x.shape, x.dtype)
+    return FP8Activations._made(codes if ld == k else codes.as_strided((m, k), (ld, 1)), scales, x.shape, x.dtype)
 
 
 def dequantize_fp8(q: FP8Weight | FP8Activations, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
