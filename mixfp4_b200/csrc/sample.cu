@@ -131,6 +131,16 @@ __device__ __forceinline__ uint32_t add_rank32(uint32_t addr, uint32_t v) {
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(was) : "r"(addr), "r"(v) : "memory");
     return was;
 }
+// The cluster's first barrier in two halves: no CTA touches a peer's shared memory before the peer is known to run, which
+// nothing but a barrier of the cluster tells.  Begun at the kernel's start, ended ahead of the first store to a peer: the row's
+// loads lie between.
+__device__ __forceinline__ void started(int ranks) {
+    if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void all_started(int ranks) {
+    __syncwarp();
+    if (ranks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void meet(int ranks) {        // all threads of the cluster; writes before are seen after
     __syncwarp();
     if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -386,6 +396,7 @@ struct Sampler {
 
     __device__ void run(int64_t r) {
         const int ranks = a.ranks;
+        started(ranks);
         // the row's granules, the cluster's share, the warps' shares: contiguous, so that indices rise with rank, warp, lane
         const int granules = (a.vocab + skew + kPer - 1) / kPer, per_rank = (granules + ranks - 1) / ranks;
         first = min(rank * per_rank, granules);
@@ -435,6 +446,7 @@ struct Sampler {
             s.warp_max[warp] = most;
             s.warp_least[warp] = least;
         }
+        all_started(ranks);
         __syncthreads();
         if (warp == 0) {
             most = s.warp_max[lane % kSampleWarps];

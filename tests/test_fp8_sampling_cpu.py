@@ -3,6 +3,8 @@ Python, and the converter's choice of layers."""
 
 import copy
 import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -152,3 +154,17 @@ def test_converter_refuses_names_that_are_no_linear():
         with pytest.raises(KeyError):
             mx.quantize_model_weights(model, "bf16", per_module_mode={name: "fp8"})
     assert mx.quantize_model_weights(model, "bf16") == []
+
+
+def test_the_sampler_meets_its_cluster_before_it_writes_to_a_peer():
+    """A peer's shared memory may be touched once the peer is known to have started: in the order of the code the cluster's first
+    barrier is complete ahead of every access to a peer's memory.  (A CTA that is not running yet cannot be had on demand.)"""
+    with open(os.path.join(os.path.dirname(mx.__file__), "csrc", "sample.cu")) as f:
+        text = f.read()
+    run = text[text.index("void run(int64_t r)"): text.index("sample_kernel(const SampleArgs a)")]
+    run = re.sub(r"//[^\n]*", "", run)
+    remote = re.search(r"\b(st_rank\d+|ld_rank\d+|add_rank\d+|find|choose_from_few)\(", run).start()
+    complete = re.search(r"\b(all_started|meet)\(", run).start()
+    assert complete < remote
+    if run[complete:].startswith("all_started"):
+        assert 0 <= run.find("started(ranks);") < run.index("griddepcontrol.wait") < complete

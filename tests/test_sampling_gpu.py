@@ -241,3 +241,13 @@ def test_logits_closer_together_than_a_bin(dtype):
             x, u = _logits(rows, vocab, dtype, 71 + k, scale)
             for settings in (dict(temperature=1.5), dict(top_p=0.5), dict(temperature=20.0, min_p=0.9)):
                 _check(x, u, top_k=k, **settings)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 16384), (12, 16384), (20, 8192), (40, 4096)])
+def test_shortest_slices_launch_after_launch(rows, vocab):
+    """CTAs of 2048 logits, eight, four and two to a row: a CTA gets to its peers' memory as early as it ever does."""
+    x, u = _logits(rows, vocab, torch.bfloat16, rows)
+    _check(x, u, top_k=50, top_p=0.9)
+    want = mx.sample_logits(x, u, top_k=50, top_p=0.9)
+    got = [mx.sample_logits(x, u, top_k=50, top_p=0.9) for _ in range(300)]
+    assert torch.equal(torch.stack(got), want.expand(300, rows))
