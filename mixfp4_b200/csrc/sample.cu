@@ -419,20 +419,22 @@ struct Sampler {
 
         float most = kNegInf;
         constexpr int kAhead = 4;                        // granules of a lane on their way at once
+        // Past the warp's share a lane takes its own last granule once more: lanes' maxima are of elements of their own.
+        const int own_last = g0 + lane + (g1 - 1 - g0 - lane) / 32 * 32;
 #pragma unroll 1
         for (int g = g0 + lane; g < g1; g += 32 * kAhead) {
             uint4 v[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) v[i] = fetch(min(g + 32 * i, g1 - 1));
+            for (int i = 0; i < kAhead; ++i) v[i] = fetch(min(g + 32 * i, own_last));
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                if constexpr (kResident) held[min(g + 32 * i, g1 - 1) - first] = v[i];
+                if constexpr (kResident) held[min(g + 32 * i, own_last) - first] = v[i];
 #pragma unroll
                 for (int j = 0; j < kPer; ++j) most = fmaxf(most, Elem<T>::load(reinterpret_cast<const T*>(&v[i]) + j));
             }
         }
-        // The largest; and the least of the maxima of so many groups of lanes that there are k of them at least: no fewer than
-        // k elements reach it, so a top-k need not look below.
+        // The largest; and the least of the maxima of so many groups of lanes that there are k of them at least.  No two groups have
+        // an element in common, so no fewer than k elements reach it, and a top-k need not look below.
         const int groups = kSampleWarps * ranks;
         float least = k <= groups * 32 ? most : kNegInf;
 #pragma unroll

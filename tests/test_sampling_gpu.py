@@ -251,3 +251,31 @@ def test_shortest_slices_launch_after_launch(rows, vocab):
     want = mx.sample_logits(x, u, top_k=50, top_p=0.9)
     got = [mx.sample_logits(x, u, top_k=50, top_p=0.9) for _ in range(300)]
     assert torch.equal(torch.stack(got), want.expand(300, rows))
+
+
+@pytest.mark.parametrize("rows,vocab,dtype,k,step", [
+    (64, 4096, torch.bfloat16, 50, 256), (1, 32768, torch.float32, 200, 256), (1, 32000, torch.bfloat16, 200, 250),
+    (1, 4096, torch.float32, 50, 128), (1, 128256, torch.bfloat16, 300, 1002), (64, 4100, torch.float16, 100, 257)])
+def test_top_k_of_rows_with_few_large_logits(rows, vocab, dtype, k, step):
+    """Fewer than k large logits, each at the end of what a warp reads: the others that belong to the first k are found below them."""
+    g = torch.Generator().manual_seed(k + vocab)
+    u = torch.rand(rows, generator=g).cuda()
+    for offset in (step - 1, 0, step // 2, step - 9):
+        x = torch.rand((rows, vocab), generator=g)
+        x[:, offset::step] = 5.0
+        x = x.to(dtype).cuda()
+        for settings in (dict(), dict(temperature=8.0), dict(temperature=4.0, top_p=0.7), dict(temperature=8.0, min_p=0.55)):
+            _check(x, u, top_k=k, **settings)
+
+
+def test_top_k_of_rows_that_rise_and_fall():
+    """Rows in order, and in runs of every length up to a warp's share: the largest stand together, wherever that is."""
+    x = torch.empty((40, 6007))
+    ramp = torch.arange(6007, dtype=torch.float32)
+    for r in range(40):
+        run = 1 + 11 * r
+        x[r] = (ramp % run) * (1 if r % 2 else -1) + ramp * 1e-5
+    x, u = (x / 40).cuda(), torch.rand(40, generator=torch.Generator().manual_seed(5)).cuda()
+    for k in (2, 17, 33, 64, 65, 130, 500, 513, 2000):
+        _check(x, u, top_k=k, temperature=3.0)
+    _check(x[:1].contiguous(), u[:1], top_k=400, temperature=3.0)
