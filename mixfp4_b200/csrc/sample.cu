@@ -40,6 +40,9 @@ constexpr int kOneLog = 44;
 constexpr double kOne = 17592186044416.0;                // 2^44
 constexpr int kSteps = 64;                               // of an octave, in the table of the exponential
 constexpr float kSpan = 31.5f;                           // weights vanish at 45 ln 2 = 31.2
+// Below 2^-160 the smallest difference of two fp32 numbers, 2^-149, is 2^11 temperatures: only the largest logits have a weight, at
+// this one as at any smaller, whose reciprocal need not be finite.
+constexpr double kLeastTemperature = 0x1p-160;
 constexpr float kNegInf = -__builtin_huge_valf();
 
 typedef unsigned long long u64;
@@ -746,6 +749,7 @@ extern "C" int mixfp4_sample(const void* logits, int dtype, int64_t rows, int64_
         return MIXFP4_E_ALIGN;
     SampleArgs a = {};
     a.logits = logits; a.ld = ld; a.vocab = (int)vocab; a.uniform = uniform;
+    if (temperature_all > 0.0 && temperature_all < kLeastTemperature) temperature_all = kLeastTemperature;
     a.temperature = {temperature, temperature_all}; a.top_k = {top_k, top_k_all};
     a.top_p = {top_p, top_p_all}; a.min_p = {min_p, min_p_all};
     a.token = reinterpret_cast<long long*>(token); a.logprob = logprob;

@@ -279,3 +279,18 @@ def test_top_k_of_rows_that_rise_and_fall():
     for k in (2, 17, 33, 64, 65, 130, 500, 513, 2000):
         _check(x, u, top_k=k, temperature=3.0)
     _check(x[:1].contiguous(), u[:1], top_k=400, temperature=3.0)
+
+
+@pytest.mark.parametrize("temperature", [5e-324, 1e-310, 3e-309, 1e-307, 1e-300, 1e-60, 1e-45])
+def test_temperatures_below_those_of_fp32(temperature):
+    """A number is a double: down to the smallest, whose reciprocal is not finite, all the weight is the largest logits'."""
+    g = torch.Generator().manual_seed(47)
+    u = torch.tensor([0.1, 0.3, 0.6, 0.9], device="cuda")
+    x = torch.randn((4, 3001), generator=g)
+    x[0, [5, 900, 2000]] = 9.0                               # three share it
+    x[1] = 1e-45 * torch.randint(0, 3, (3001,), generator=g)      # neighbours of the smallest size
+    x[2, 17] = 3e38
+    x[3] = x[3].abs().neg() * 1e-38
+    for kind in (torch.float32, torch.bfloat16):
+        for settings in (dict(), dict(top_k=2), dict(top_k=700), dict(top_p=0.6), dict(min_p=0.5), dict(top_k=2000, top_p=0.99)):
+            _check(x.to(kind).cuda(), u, temperature=temperature, **settings)
