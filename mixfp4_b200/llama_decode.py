@@ -92,8 +92,8 @@ class Decoder:
             stack = [Layer(i, device, gen, rank, world) for i in range(layers)]
             gen.manual_seed(99)
             embed = (torch.randn((VOCAB, HIDDEN), generator=gen, device=device) * 0.02).to(torch.bfloat16)
-            head = (torch.randn((VOCAB, HIDDEN), generator=gen, device=device) * 0.02).to(torch.bfloat16)
-            weights = (stack, embed, head)
+            unembed = (torch.randn((VOCAB, HIDDEN), generator=gen, device=device) * 0.02).to(torch.bfloat16)
+            weights = (stack, embed, unembed)
         self.weights = weights
         self.layers, self.embed, self.head = weights
         self.head_fp8 = mx.quantize_fp8_weight(self.head) if head == "fp8" else None

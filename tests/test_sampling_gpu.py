@@ -294,3 +294,23 @@ def test_temperatures_below_those_of_fp32(temperature):
     for kind in (torch.float32, torch.bfloat16):
         for settings in (dict(), dict(top_k=2), dict(top_k=700), dict(top_p=0.6), dict(min_p=0.5), dict(top_k=2000, top_p=0.99)):
             _check(x.to(kind).cuda(), u, temperature=temperature, **settings)
+
+
+def test_decoder_runs_the_head_that_it_was_asked_for(monkeypatch):
+    from mixfp4_b200 import llama_decode
+
+    device, norms = torch.device("cuda", torch.cuda.current_device()), []
+    norm = llama_decode.rms_norm
+    monkeypatch.setattr(llama_decode, "rms_norm", lambda *args: norms.append(norm(*args)) or norms[-1])
+    fp8 = llama_decode.Decoder(1, 2, 16, device, head="fp8")
+    plain = llama_decode.Decoder(1, 2, 16, device, weights=fp8.weights)
+    again = llama_decode.Decoder(1, 2, 16, device, weights=fp8.weights, head="fp8")
+    ids = torch.randint(0, llama_decode.VOCAB, (2, 9), generator=torch.Generator().manual_seed(3)).to(device)
+    with torch.no_grad():
+        for model, quantized in ((fp8, True), (plain, False), (again, True)):
+            assert (model.head_fp8 is not None) == quantized
+            logits = model.forward(ids, torch.arange(9, device=device), 9)
+            last = norms[-1]
+            assert torch.equal(logits, mx.fp8_linear(last, mx.quantize_fp8_weight(model.head)) if quantized else last @ model.head.T)
+    with pytest.raises(ValueError):
+        llama_decode.Decoder(1, 2, 16, device, weights=fp8.weights, head="fp4")
