@@ -207,16 +207,16 @@ def run(layers: int = 32, batch: int = 1, prompt: int = 2048, tokens: int = 32, 
     assert torch.isfinite(logits).all()
     # decode: one token per sequence at the position after the prompt, cache length prompt + 1
     pos = torch.tensor([prompt], device=device)
+    forward = step = lambda: model.forward(nxt, pos, prompt + 1)
     if sampling is None:
         nxt = logits.argmax(-1, keepdim=True)
-        step = lambda: model.forward(nxt, pos, prompt + 1)
     else:
         uniform = torch.rand(batch, generator=gen, device=device)        # the same on every rank
         nxt = mx.sample_logits(logits, uniform, **sampling)[:, None]
-        step = lambda: mx.sample_logits(model.forward(nxt, pos, prompt + 1), uniform, **sampling)
+        step = lambda: mx.sample_logits(forward(), uniform, **sampling)
     full_ms = _time_graph(step, tokens)
     model.linears_only = True
-    lin_ms = _time_graph(step, tokens)
+    lin_ms = _time_graph(forward, tokens)
     model.linears_only = False
     if tp > 1:
         t = torch.tensor([prefill_ms, full_ms, lin_ms], device=device, dtype=torch.float64)

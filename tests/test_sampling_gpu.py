@@ -314,3 +314,21 @@ def test_decoder_runs_the_head_that_it_was_asked_for(monkeypatch):
             assert torch.equal(logits, mx.fp8_linear(last, mx.quantize_fp8_weight(model.head)) if quantized else last @ model.head.T)
     with pytest.raises(ValueError):
         llama_decode.Decoder(1, 2, 16, device, weights=fp8.weights, head="fp4")
+
+
+def test_harness_times_the_linears_without_the_sampler(monkeypatch):
+    from mixfp4_b200 import llama_decode
+
+    drawn, per_step = [], []
+    sample = mx.sample_logits
+    monkeypatch.setattr(mx, "sample_logits", lambda *args, **kwargs: drawn.append(1) or sample(*args, **kwargs))
+
+    def step_once(fn, steps):
+        before = len(drawn)
+        fn()
+        per_step.append(len(drawn) - before)
+        return 1.0
+
+    monkeypatch.setattr(llama_decode, "_time_graph", step_once)
+    llama_decode.run(layers=1, batch=1, prompt=8, tokens=1, sampling={"temperature": 0.8})
+    assert per_step == [1, 0]                                # a whole step, the linears alone
