@@ -249,6 +249,8 @@ def main() -> None:
     ap.add_argument("--top-p", type=float, default=1.0)
     ap.add_argument("--min-p", type=float, default=0.0)
     args = ap.parse_args()
+    if args.temperature is None and (args.top_k, args.top_p, args.min_p) != (0, 1.0, 0.0):
+        ap.error("--top-k, --top-p and --min-p filter tokens that are drawn: they need --temperature")
     sampling = None if args.temperature is None else {"temperature": args.temperature, "top_k": args.top_k, "top_p": args.top_p, "min_p": args.min_p}
     local = int(os.environ.get("LOCAL_RANK", "0"))
     torch.cuda.set_device(local)

@@ -11,6 +11,7 @@ import torch
 
 import mixfp4_b200 as mx
 from mixfp4_b200 import _native as nat
+from mixfp4_b200 import llama_decode
 
 ONE = ctypes.c_void_p(64)       # never dereferenced: validation fails first
 ODD = ctypes.c_void_p(66)
@@ -168,3 +169,12 @@ def test_the_sampler_meets_its_cluster_before_it_writes_to_a_peer():
     assert complete < remote
     if run[complete:].startswith("all_started"):
         assert 0 <= run.find("started(ranks);") < run.index("griddepcontrol.wait") < complete
+
+
+@pytest.mark.parametrize("filters", [["--top-k", "50"], ["--top-p", "0.9"], ["--min-p", "0.1"], ["--top-k", "0", "--top-p", "0.5"]])
+def test_harness_refuses_filters_without_a_temperature(filters, monkeypatch, capsys):
+    """Without a temperature no token is drawn: a filter would be dropped in silence."""
+    monkeypatch.setattr("sys.argv", ["llama_decode", *filters])
+    with pytest.raises(SystemExit):
+        llama_decode.main()
+    assert "--temperature" in capsys.readouterr().err
