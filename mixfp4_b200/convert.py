@@ -28,7 +28,7 @@ from torch import nn
 
 from .fp8 import FP8Linear, FP8Weight
 from .linear import MixFP4Linear
-from .quant import PackedWeight
+from .quant import HIGH_PRECISION_MODES, PackedWeight, _packable
 
 FORMAT_NAME = "mixfp4_b200.packed"
 FORMAT_VERSION = 1
@@ -86,10 +86,14 @@ def quantize_model_weights(model: nn.Module, weight_mode: str = "oracle16", *, r
         if not isinstance(modules.get(name), nn.Linear):
             raise KeyError(f"per_module_mode names {name!r}, which is not a linear of the model")
         linears.setdefault(name, modules[name])
+    modes = {name: own_mode.get(name, weight_mode) for name in linears}
+    for mode in modes.values():                      # before the first layer is replaced
+        if mode != "fp8" and mode not in HIGH_PRECISION_MODES and not _packable(mode):
+            raise ValueError(f"unsupported mode {mode!r}")
     rows = []
     for name, linear in linears.items():
-        mode = own_mode.get(name, weight_mode)
-        if mode in {"high_precision", "fp16", "bf16"}:
+        mode = modes[name]
+        if mode in HIGH_PRECISION_MODES:
             continue
         if mode == "fp8":
             layer = FP8Linear.from_linear(linear, device=device)

@@ -272,6 +272,11 @@ def _as_rows(x: torch.Tensor) -> torch.Tensor:
     return x2
 
 
+def _packable(mode: str) -> bool:
+    """Whether `quantize_packed` has this mode."""
+    return mode in _MODE_CODE or mode in _WEIGHT_REGIONS or mode in _ACTIVATION_REGIONS
+
+
 def quantize_packed(x: torch.Tensor, *, mode: str = "oracle16", amax: torch.Tensor | None = None,
                     want_dequant: bool = False, want_stats: bool = False, rotation: str | None = None,
                     region: tuple[int, int] | None = None):

@@ -178,3 +178,15 @@ def test_harness_refuses_filters_without_a_temperature(filters, monkeypatch, cap
     with pytest.raises(SystemExit):
         llama_decode.main()
     assert "--temperature" in capsys.readouterr().err
+
+
+def test_converter_refuses_modes_before_it_converts():
+    """A mode that does not exist, wherever it stands: no layer ahead of it has been replaced."""
+    for args, kwargs in ((("oracle16",), dict(per_module_mode={"2": "fp4"})), (("fp9",), {}), (("fp9",), dict(per_module_mode={"0": "fp8"})),
+                         (("fp8",), dict(per_module_mode={"2": "oracle17"}))):
+        model = torch.nn.Sequential(torch.nn.Linear(16, 16), torch.nn.ReLU(), torch.nn.Linear(16, 16))
+        held = list(model)
+        with pytest.raises(ValueError, match="unsupported mode"):
+            mx.quantize_model_weights(model, *args, **kwargs)
+        assert all(a is b for a, b in zip(model, held))
+    assert mx.quantize_model_weights(model, "fp9", per_module_mode={"0": "bf16", "2": "fp16"}) == []     # a mode that no layer takes
