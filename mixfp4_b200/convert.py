@@ -9,12 +9,12 @@ bytes (and rotates its input itself), and the packed bytes can be written to and
 checkpoint file, so a model is quantized once.
 
 Checkpoint format (`torch.save` of plain tensors and python scalars, no code objects):
-    {"format": "mixfp4_b200.packed", "version": 1, "layers": {module name: {
+    {"format": "mixfp4_b200.packed", "version": 1 or 2, "layers": {module name: {
         "codes": u8 [n, kpad/2], "scales": u8 [n, kpad/16], "fmt": u8 [n, kpad/128],
         "global_scale": f32 [1], "n": int, "k": int, "rotation": str | None, "mode": str,
         "activation_mode": str | None, "bias": tensor | None}}}
 The bytes are the canonical layout of include/mixfp4_b200.h (the one the parity tests hash);
-the kernel layout and the decode tables are rebuilt at load time.  A layer in block-scaled FP8 has instead
+the kernel layout and the decode tables are rebuilt at load time.  Version 2 has layers in block-scaled FP8 too, of the form
     {"mode": "fp8", "codes": u8 [n, k] (E4M3), "scales": f32 [ceil(n/128), ceil(k/128)], "n": int, "k": int, "bias": tensor | None}
 """
 
@@ -31,7 +31,7 @@ from .linear import MixFP4Linear
 from .quant import HIGH_PRECISION_MODES, PackedWeight, _packable
 
 FORMAT_NAME = "mixfp4_b200.packed"
-FORMAT_VERSION = 1
+FORMAT_VERSION, FORMAT_VERSION_FP8 = 1, 2          # without and with layers in block-scaled FP8
 LINEAR_TYPES = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
 
 
@@ -140,7 +140,8 @@ def packed_state(model: nn.Module) -> dict[str, Any]:
                 "n": module.out_features, "k": module.in_features,
                 "bias": None if module.bias is None else module.bias.detach().cpu(),
             }
-    return {"format": FORMAT_NAME, "version": FORMAT_VERSION, "layers": layers}
+    version = FORMAT_VERSION_FP8 if any(e["mode"] == "fp8" for e in layers.values()) else FORMAT_VERSION
+    return {"format": FORMAT_NAME, "version": version, "layers": layers}
 
 
 def save_packed(model: nn.Module, path: str) -> None:
@@ -154,7 +155,7 @@ def load_packed(model: nn.Module, path_or_state, *, device=None, strict: bool = 
     were installed; with strict=True a checkpoint layer without a module of that name, or a
     shape mismatch, raises."""
     state = torch.load(path_or_state, map_location="cpu", weights_only=True) if isinstance(path_or_state, str) else path_or_state
-    if state.get("format") != FORMAT_NAME or state.get("version") != FORMAT_VERSION:
+    if state.get("format") != FORMAT_NAME or state.get("version") not in (FORMAT_VERSION, FORMAT_VERSION_FP8):
         raise ValueError("not a mixfp4_b200 packed checkpoint of a known version")
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     modules = dict(model.named_modules())

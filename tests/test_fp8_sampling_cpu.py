@@ -11,7 +11,7 @@ import torch
 
 import mixfp4_b200 as mx
 from mixfp4_b200 import _native as nat
-from mixfp4_b200 import llama_decode
+from mixfp4_b200 import convert, llama_decode
 
 ONE = ctypes.c_void_p(64)       # never dereferenced: validation fails first
 ODD = ctypes.c_void_p(66)
@@ -190,3 +190,20 @@ def test_converter_refuses_modes_before_it_converts():
             mx.quantize_model_weights(model, *args, **kwargs)
         assert all(a is b for a, b in zip(model, held))
     assert mx.quantize_model_weights(model, "fp9", per_module_mode={"0": "bf16", "2": "fp16"}) == []     # a mode that no layer takes
+
+
+def test_checkpoints_with_fp8_layers_carry_a_version_of_their_own():
+    """A reader that knows packed layers alone refuses the whole file instead of failing at such an entry, half-way through the model."""
+    weight = mx.FP8Weight.from_tensors(torch.randint(0, 100, (200, 300), dtype=torch.uint8), torch.rand((2, 3)))
+    model = torch.nn.Sequential(torch.nn.Linear(300, 200), mx.FP8Linear(weight, torch.rand(200)))
+    state = convert.packed_state(model)
+    assert state["version"] == 2 and list(state["layers"]) == ["1"]
+    assert convert.packed_state(torch.nn.Sequential(torch.nn.ReLU()))["version"] == 1
+    for version in (1, 2):                                   # 1: as such checkpoints were written at first
+        other = torch.nn.Sequential(torch.nn.Linear(300, 200), torch.nn.Linear(300, 200))
+        assert mx.load_packed(other, dict(state, version=version), device="cpu") == ["1"]
+        assert torch.equal(other[1].codes.view(torch.uint8), model[1].codes.view(torch.uint8))
+        assert torch.equal(other[1].scales, model[1].scales) and torch.equal(other[1].bias, model[1].bias)
+    for version in (0, 3, None):
+        with pytest.raises(ValueError, match="version"):
+            mx.load_packed(other, dict(state, version=version), device="cpu")
