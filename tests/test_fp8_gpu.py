@@ -348,3 +348,36 @@ def test_outputs_past_2_31_elements():
     a, b = _expand(q.codes, q.scales, 1), _expand(weight.codes, weight.scales, 128)
     for rows, cols in ((slice(0, 3), slice(0, n)), (slice(m - 3, m), slice(0, n)), (slice(0, m), slice(n - 5, n))):
         _check_product(y[rows, cols], a[rows], b[cols], torch.bfloat16)
+
+
+def _kernels(call):
+    """What `call` returns, and the names of the kernels that it launched (none where the profiler is not to be had)."""
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA], acc_events=True) as prof:
+        result = call()
+        torch.cuda.synchronize()
+    return result, [e.name for e in prof.events() if e.device_type == torch.autograd.DeviceType.CUDA]
+
+
+@pytest.mark.parametrize("m,n,k,out,kernel", [
+    (4096, 4099, 4096, torch.bfloat16, "fp8_pair_kernel"), (4096, 4099, 4096, torch.float32, "fp8_pair_kernel"),
+    (2048, 4096, 4096, torch.bfloat16, "fp8_pair_kernel"), (2000, 4112, 4000, torch.float16, "fp8_pair_kernel"),
+    (5000, 8200, 1100, torch.float32, "fp8_pair_kernel"), (1100, 8976, 2944, torch.bfloat16, "fp8_pair_kernel"),
+    (1100, 9000, 2944, torch.bfloat16, "fp8_gemm_kernel<128, false, false>")])       # off its sectors pairs cost more
+def test_many_blocks_and_tiles(m, n, k, out, kernel):
+    """256 x 256 tiles of CTA pairs: their ring of stages wraps within a tile, a pair takes several tiles one after the other (4096 x 4099:
+    272 tiles for 74 pairs), K ends inside a block, rows of y on their sectors and off them.  The kernel's name says that a case is still
+    what it stands for."""
+    x, w = _data(m, k, torch.bfloat16, m + k), _data(n, k, torch.bfloat16, n + k)
+    q, weight = mx.quantize_fp8_activations(x), mx.quantize_fp8_weight(w)
+    y, names = _kernels(lambda: mx.fp8_linear(q, weight, out_dtype=out))
+    assert not names or any(kernel in name for name in names), names
+    a, b = _expand(q.codes, q.scales, 1), _expand(weight.codes, weight.scales, 128)
+    # What rounds to infinity is what lies half a step past the largest value: fp16 holds 65504, its next step would be 65536, so
+    # everything below 65520 is 65504.  The sum's own error moves that border.
+    largest = torch.finfo(out).max
+    border = largest * (1 + HALF_STEP[out] / (2 - 2 * HALF_STEP[out]))      # (2 - 2h) 2^e is the largest, h 2^e half a step there
+    ref, room = a @ b.T, (2 * 128 + -(-k // 128) + 4) * 2.0 ** -24 * (a.abs() @ b.abs().T)
+    over = y.isinf()
+    assert (ref[over].abs() + room[over] >= border).all() and ((y[over] > 0) == (ref[over] > 0)).all()
+    assert ((y.double() - ref).abs()[~over] <= (room + HALF_STEP[out] * ref.abs() + SUBNORMAL[out])[~over]).all()
+    assert torch.equal(mx.fp8_linear(x, weight, out_dtype=out), y) and mx.gemm_status() == 0
