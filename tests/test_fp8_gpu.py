@@ -381,3 +381,25 @@ def test_many_blocks_and_tiles(m, n, k, out, kernel):
     assert (ref[over].abs() + room[over] >= border).all() and ((y[over] > 0) == (ref[over] > 0)).all()
     assert ((y.double() - ref).abs()[~over] <= (room + HALF_STEP[out] * ref.abs() + SUBNORMAL[out])[~over]).all()
     assert torch.equal(mx.fp8_linear(x, weight, out_dtype=out), y) and mx.gemm_status() == 0
+
+
+def test_tiles_and_columns_around_2_31_elements():
+    """Codes and scales past element 2^31 (row 524288) are those of the rows by themselves, and so are the columns of a product."""
+    n, k = 530000, 4096
+    dense = torch.empty((n, k), dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(81))
+    weight = mx.quantize_fp8_weight(dense)
+    parts = {}
+    for first, last in ((524288 - 128, 524288 + 128), (n - 208, n)):              # whole tiles: 530000 = 4139 * 128 + 208
+        part = parts[first, last] = mx.quantize_fp8_weight(dense[first:last])
+        assert torch.equal(weight.codes[first:last].view(torch.uint8), part.codes.view(torch.uint8))
+        assert torch.equal(weight.scales[first // 128: -(-last // 128)], part.scales)
+        for out in (torch.bfloat16, torch.float32):
+            assert torch.equal(weight.dequantize(out)[first:last], part.dequantize(out))
+    for m in (1, 70, 300):
+        x = _data(m, k, torch.bfloat16, 82 + m, spread=False)
+        q = mx.quantize_fp8_activations(x)
+        y, a = mx.fp8_linear(x, weight), _expand(q.codes, q.scales, 1)
+        for (first, last), part in parts.items():
+            b = _expand(part.codes, part.scales, 128)
+            _check_product(y[:, first:last], a, b, torch.bfloat16)
+            _check_product(mx.fp8_linear(x, part), a, b, torch.bfloat16)
