@@ -16,9 +16,10 @@
 //   warp E           producer: per block of 128 K a box of both operands (128-byte swizzle) and the scales of x
 //   warp E + 1       tensor memory, MMA issue
 //
-// What bounds it.  One token, 128256 x 4096: HBM (79 us, 6.6 TB/s).  Few rows: a fixed 5 to 6 us (launch, set-up, first loads,
-// exchange) beside the weights' bytes; 48 x 14336 x 4096 also that 112 tiles keep 112 of 148 SMs busy (15.7 us, 3.8 TB/s).
-// Many rows: 4096 x 14336 x 4096 242 us, 1.99 PFLOP/s, in a burst and 284 us under the power cap; a block takes about 1060 cycles
+// What bounds it.  One token, 128256 x 4096: HBM (79 us, 6.7 TB/s).  Few rows: a fixed 5 to 6 us (launch, set-up, first loads,
+// exchange) beside the weights' bytes; 48 x 14336 x 4096 (15.7 us, 3.8 TB/s) also that items are whole tiles, so that its 112 keep 112 of
+// 148 SMs busy: a choice of this split, not a limit (tiles cut along K between neighbouring clusters would use all).
+// Many rows: 4096 x 14336 x 4096 242 us, 1.99 PFLOP/s, in a burst and 284 us under the power cap (1.67 GHz); a block takes about 1060 cycles
 // of a pair for 512 of MMA, the rest is the way of a buffer from the MMA's end through the epilogue back to the issuer.
 //
 // Work split: an item is a tile of y.  A cluster of c CTAs (1, 2, 4 or 8) takes items in turn; its CTAs cut the blocks of K

@@ -5,7 +5,7 @@
 // The scale is held in fp32; one that would be zero (a block of zeros, or of magnitudes below 448 times the smallest
 // subnormal) becomes 1.  A block that holds a NaN or an infinity has that as its scale, and NaN codes.
 //
-// Both passes read a block once, keep it in registers and write codes and scale from there: bound by HBM.
+// Both passes read a block once, keep it in registers and write codes and scale from there.
 
 #include "common.cuh"
 #include "fp8.cuh"
@@ -13,9 +13,10 @@
 namespace mixfp4 {
 namespace {
 
-// A group of eight lanes per row and block (4096 x 4096 bf16: 11.4 us, 4.4 TB/s, bound by instruction issue as much as by loads; two
-// blocks a group with their loads ahead 12.1 to 16.4, four 14.3; with 64-bit indices 12.1).  scales: [block][lds], a row's scales a column of it, so that the product reads
-// the scales of neighbouring rows together.
+// A group of eight lanes per row and block (4096 x 4096 bf16: 10.5 to 11.4 us, 4.4 to 4.8 TB/s; issue slots 70 % busy, 15 thread
+// instructions an element: fewer are possible, by indices that are carried along instead of
+// divided and by paired fp32 operations; two blocks a group with their loads ahead 12.1 to 16.4, four 14.3; with 64-bit indices 12.1).
+// scales: [block][lds], a row's scales a column of it, so that the product reads the scales of neighbouring rows together.
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_rows_kernel(const T* x, uint32_t total, uint32_t blocks, int64_t k, int64_t ldx, bool vec,
                                                        uint8_t* codes, int64_t ldq, float* scales, int64_t lds) {
@@ -42,8 +43,8 @@ __global__ void __launch_bounds__(256) fp8_rows_kernel(const T* x, uint32_t tota
     }
 }
 
-// A CTA of 256 threads per 128 x 128 tile: 32 rows a pass, four passes, 64 elements a thread, kept as they were read: in 16 bits
-// four CTAs fit an SM, and the loads of one hide behind the arithmetic of the others (14336 x 4096 bf16: 33 us, 5.3 TB/s;
+// Bound by HBM.  A CTA of 256 threads per 128 x 128 tile: 32 rows a pass, four passes, 64 elements a thread, kept as they were read: in 16 bits
+// four CTAs fit an SM, and the loads of one hide behind the arithmetic of the others (14336 x 4096 bf16: 31 us, 5.7 TB/s;
 // elements kept in fp32 by 512 threads, two CTAs an SM, 49 us; 512 threads and three CTAs 38 us; five CTAs of 256, 39 us).
 // Rows off their 16 bytes are read an element at a time: 14333 x 4095 bf16 61 us, fp32 98 us (aligned 31 and 50).
 constexpr int kTileThreads = 256, kTilePasses = 128 * kLanesPerRow / kTileThreads;
@@ -81,7 +82,9 @@ __global__ void __launch_bounds__(kTileThreads, sizeof(T) == 2 ? 4 : 2) fp8_tile
     }
 }
 
-// y = code * scale, rounded once.  One thread per 4 columns.
+// y = code * scale, rounded once.  One thread per 4 columns, an element at a time: a form for checks and exports, simple rather than
+// fast (14336 x 4096 to bf16 112 us, 1.6 TB/s, to fp32 123 us; its bytes alone 27 and 45 us at the copy rate; bound by instruction
+// issue, 82 % of the slots, 57 thread instructions an element).
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_dequant_kernel(const uint8_t* codes, int64_t ldq, const float* scales,
                                                           int64_t row_stride, int64_t block_stride, int rows_per_scale,

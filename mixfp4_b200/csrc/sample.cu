@@ -19,11 +19,13 @@
 //
 // What bounds it.  A row of a small batch takes a dozen dependent steps (passes over shared memory, cluster barriers), and code
 // that runs once or twice: instruction fetch counts, so every pass has one copy (unrolled passes, 86 KB of code, took 70 us for
-// one row of 128256 logits with top-k and top-p; this takes 13).  Large batches: the fp64 operations of the weights, in a pass
-// with all of them 14 us for the 64 K elements of an SM, and the histogram's additions in shared memory.
+// one row of 128256 logits with top-k and top-p; this takes 12 to 13).  Large batches without a top-k (64 mixed rows of 128256 57 to 61
+// us): instruction issue, 166 thread instructions a logit of a top-p, of which the weights are about half.  They are computed in fp64 for
+// every logit, once for the histogram and once for the sums (a pass with all of them 14 us for the 64 K elements of an SM), although
+// logits of 16 bits have a few thousand values: fewer are possible.  The rest are the histogram's additions in shared memory.
 // Measured and not kept: lists of a warp's few elements of interest, sorting the candidates, sums of what a top-p cannot reach
 // beside the histogram, a first histogram over the topmost bf16 keys instead of equal widths (each more code than it saved time:
-// 64 mixed rows 61 to 65 us, so 69 to 79).
+// 64 mixed rows 4 to 14 us more).
 
 #include <float.h>
 
@@ -699,7 +701,7 @@ int launch_sample(const SampleArgs& a, int64_t rows, size_t smem, cudaStream_t s
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     // One that starts under the tail of the kernel before gets the SMs in the order in which they fall free, two CTAs to each:
-    // only where every CTA would have an SM to itself anyway (64 rows of 128256, 256 CTAs: 61 us without, 67 us with it).
+    // only where every CTA would have an SM to itself anyway (64 mixed rows of 128256, 256 CTAs: 61 us without, 67 us with it).
     cfg.attrs = attr;
     cfg.numAttrs = rows * a.ranks <= 148 ? 2 : 1;
     const auto kernel = sample_kernel<T, kResident>;

@@ -3,7 +3,10 @@
     activations   E4M3 codes and one fp32 scale for every row and 128 columns
     weights       E4M3 codes and one fp32 scale for every 128 x 128 tile
     scale         the block's largest magnitude / 448 (1 where that is zero); code = e4m3(fp32(value / scale))
-    y[m, n]     = sum over blocks b of sx[m, b] * sw[n // 128, b] * (sum of code products in b), in fp32, rounded once
+    y[m, n]     = sum over blocks b of (sx[m, b] * sw[n // 128, b]) * (sum of code products in b), in fp32, rounded once
+
+The two scales are multiplied first, in fp32: blocks whose product of scales leaves its range do so too (largest magnitude of x times
+that of the weight above 6.8e43; below 2.4e-33 it loses bits).  A bias is added to the rounded y, in y's type, as `mixfp4_linear` does.
 
 The reference keeps such layers in bf16 (project_quant/modeling.py:65-68 leaves output heads out of the walk); there is no
 counterpart of this format in it.  Inputs that are not finite make their block's scale, and the results that read it, NaN.
@@ -227,8 +230,9 @@ def _workspace_bytes(m: int, k: int) -> int:
 def fp8_linear(x: torch.Tensor | FP8Activations, weight: FP8Weight, *, bias: torch.Tensor | None = None,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y = x @ W^T (+ bias) on block-scaled FP8 operands.  x: a dense tensor [..., K] (bf16, f16 or fp32), quantized within
-    the call, or what `quantize_fp8_activations` made of one.  out_dtype: bf16, f16 or fp32 (default: x's dtype).  A product
-    whose device-side waits run out reports through `gemm_status()`, like the other GEMMs."""
+    the call, or what `quantize_fp8_activations` made of one.  out_dtype: bf16, f16 or fp32 (default: x's dtype).  bias [n]: rounded
+    to that type and added to the rounded product, so a biased result is rounded twice (out_dtype=torch.float32 leaves the
+    rounding to the caller).  A product whose device-side waits run out reports through `gemm_status()`, like the other GEMMs."""
     codes, n, k = weight.codes, weight.n, weight.k
     device, shape = codes.device, x.shape
     out_dtype = x.dtype if out_dtype is None else out_dtype
